@@ -17,8 +17,8 @@
 
 #include "../../include/dcnv2.h"
 #include "../../include/dcnv2_diag.h"
-#include <cudaTypedefs.h>
 #include "dcnv2_head_kernel.cuh"
+#include "dcnv2_host.cuh"
 #include "dcnv2_kernels.cuh"
 #include "dcnv2_ta_kernel.cuh"
 
@@ -26,40 +26,7 @@ namespace dcnv2 {
 
 namespace {
 
-constexpr size_t kSmemLimit = 227 * 1024;     // opt-in dynamic shared memory per block
 constexpr size_t kErrBytes = 256;
-constexpr unsigned long long kDefaultTimeoutNs = 2000000000ull;  // 2 s per on-chip wait
-
-struct DevInfo {
-  int sm_count = 0;
-  int major = 0;
-  int minor = 0;
-  bool ok = false;
-  std::atomic<uint32_t> attr_set{0};
-  std::atomic<int> pair_clusters[3] = {{0}, {0}, {0}};  // co-resident CTA pairs, per precision
-};
-constexpr int kMaxDevices = 64;
-DevInfo g_dev[kMaxDevices];
-std::once_flag g_dev_once[kMaxDevices];
-
-DevInfo* device_info(int dev) {
-  if (dev < 0 || dev >= kMaxDevices) return nullptr;
-  std::call_once(g_dev_once[dev], [dev]() {
-    DevInfo& d = g_dev[dev];
-    if (cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, dev) != cudaSuccess) {
-      cudaGetLastError();
-      d.ok = false;
-      return;
-    }
-    d.ok = true;
-  });
-  return &g_dev[dev];
-}
-
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // Kernel-selection overrides for measurements and tests. They are read from the environment
 // once per process (DCNV2_KERNEL=ta|smem, DCNV2_PAIR=1|0) and can be changed afterwards only
 // through dcnv2_diag_set_kernel_override; the dispatch itself never calls getenv.
@@ -79,22 +46,6 @@ void read_env_overrides() {
   });
 }
 
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link needed).
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, []() {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault,
-                                         &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    cudaGetLastError();
-  });
-  return fn;
-}
-
 // Optional CUDA events recorded between the launches of one forward (diagnostics only).
 struct Marks {
   void* const* ev = nullptr;
@@ -104,7 +55,6 @@ struct Marks {
     if (ev && i < n) cudaEventRecord(static_cast<cudaEvent_t>(ev[i++]), st);
   }
 };
-inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 enum Kind { KIND_SIMT = 0, KIND_TCGEN05 = 1, KIND_F32_EXACT = 2 };
 

@@ -26,6 +26,7 @@
 #include <stdint.h>
 
 #include "../../include/dcnv2.h"
+#include "dcnv2_wait.cuh"
 #include "ptx_sm100.cuh"
 
 namespace dcnv2 {
@@ -100,45 +101,6 @@ struct FusedArgs {
                            // stores of y)
   unsigned long long timeout_ns;
 };
-
-// ------------------------------------------------------------------ bounded mbarrier wait
-// Waits for the phase of `bar` with the given parity. Gives up after timeout_ns (sets the CTA
-// abort flag and the device error word) or as soon as another role of this CTA has aborted;
-// both are checked every 16 tries so that a waiting warp issues few instructions.
-// SLEEP_NS > 0 adds a nanosleep between tries; SLEEP_NS < 0 (kSuspend) lets the hardware suspend
-// the thread until the phase completes; 0 spins (the MMA issuer, whose wake-up latency is on the
-// critical path). Waiting warps that do not spin leave the issue slots to the working ones.
-// CL selects a cluster-scope acquire (barriers that the peer CTA of a pair arrives on).
-constexpr int kSuspend = -1;
-struct WaitCtx {
-  unsigned long long timeout_ns;
-  int* err;                  // device error word
-  volatile int* abort_flag;  // this CTA's abort flag (shared memory)
-};
-template <int SLEEP_NS = 0, bool CL = false>
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const WaitCtx& w,
-                                         int code) {
-  if (CL ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = ptx::global_timer_ns();
-  for (uint32_t n = 1;; ++n) {
-    if constexpr (SLEEP_NS > 0) __nanosleep(static_cast<unsigned>(SLEEP_NS));
-    if constexpr (CL) {
-      if (ptx::mbar_try_wait_cluster(bar, parity)) return true;
-    } else if constexpr (SLEEP_NS < 0) {
-      if (ptx::mbar_try_wait_sleep(bar, parity, 1000000u)) return true;
-    } else {
-      if (ptx::mbar_try_wait(bar, parity)) return true;
-    }
-    if ((n & 15u) == 0) {
-      if (*w.abort_flag) return false;
-      if (ptx::global_timer_ns() - t0 > w.timeout_ns) {
-        *w.abort_flag = 1;
-        atomicOr(w.err, code);
-        return false;
-      }
-    }
-  }
-}
 
 __device__ __forceinline__ void decode_tile(const FusedArgs& a, int tile, int& img, int& pt,
                                             int& cc) {
