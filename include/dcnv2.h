@@ -41,11 +41,13 @@ extern "C" {
 /* Opaque CUDA stream (cudaStream_t); 0 is the legacy default stream. */
 typedef void* dcnv2_stream_t;
 
-/* Element types. Values equal nvinfer1::DataType (kFLOAT=0, kHALF=1, kINT8=2). */
+/* Element types. Values equal nvinfer1::DataType (kFLOAT=0, kHALF=1, kINT8=2, kBF16=7). BF16 is a
+ * type of the token operators only; the layer refuses it. */
 typedef enum {
   DCNV2_FLOAT = 0,
   DCNV2_HALF = 1,
-  DCNV2_INT8 = 2
+  DCNV2_INT8 = 2,
+  DCNV2_BF16 = 7
 } dcnv2_dtype;
 
 /* Tensor formats. Value equals nvinfer1::TensorFormat::kLINEAR. */
@@ -209,6 +211,93 @@ DCNV2_API int32_t dcnv2_uses_tensor_cores(const dcnv2_desc* desc);
 DCNV2_API int32_t dcnv2_launch_count(const dcnv2_desc* desc);
 
 DCNV2_API const char* dcnv2_status_string(dcnv2_status status);
+
+/* ---- Token operators: what a transformer does with the layer's feature maps ---- */
+
+/* Norms of dcnv2_qk_norm_rotary (dcnv2_rotary_desc.norm). */
+enum {
+  DCNV2_NORM_NONE = 0,
+  DCNV2_NORM_RMS = 1             /* x * rsqrt(mean(x^2) + eps) * weight, per head */
+};
+
+/* Queries and keys of `tokens` tokens each of `batch` sequences. Strides are in elements, in the
+ * order batch, token, head; the elements of a head are contiguous. */
+typedef struct {
+  int32_t batch, tokens;
+  int32_t q_heads, k_heads;      /* 0: that tensor is absent (its pointers are not read) */
+  int32_t head_dim;              /* even, at most 256 */
+  int32_t rotary_dim;            /* even, at most head_dim; elements from it on are not rotated */
+  int32_t axes;                  /* position axes, 1 to 4 (unused when rotary_dim is 0) */
+  int32_t dtype;                 /* DCNV2_FLOAT, DCNV2_HALF or DCNV2_BF16: inputs, weights, outputs */
+  int32_t norm;                  /* DCNV2_NORM_* */
+  int32_t interleaved;           /* 0: pair p is elements (p, p + rotary_dim/2); 1: (2p, 2p + 1) */
+  float eps;                     /* of the norm, >= 0 */
+  uint8_t pair_axis[128];        /* axis whose position turns pair p, for p < rotary_dim/2 */
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+  int64_t pos_batch_stride;      /* elements; 0: the sequences share their positions */
+} dcnv2_rotary_desc;
+
+/* Norm of each query and key head and its rotation by the token's position, in one pass:
+ * y = norm(x); for rotated pair p of elements (e0, e1) and a = positions[b][t][pair_axis[p]] *
+ * freqs[p]: out[e0] = y[e0] cos a - y[e1] sin a, out[e1] = y[e1] cos a + y[e0] sin a; the other
+ * elements are y. One axis is a text, two a feature map (row, column), three a video or the levels
+ * of a pyramid. fp32 arithmetic (angles reduced in fp64), one rounding.
+ *   positions  int32 [batch][tokens][axes], any values; freqs  fp32 [rotary_dim/2] (both may be
+ *   NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL (ones;
+ *   read only with DCNV2_NORM_RMS).
+ * An output may be its own input (same pointer and strides); other overlaps are not supported.
+ * Works at any element alignment, fastest where pointers, strides and dims allow 16-byte accesses.
+ * All pointers are device pointers of the current device. Asynchronous on `stream`; needs no
+ * workspace; batch or tokens 0 is a no-op. No counterpart in the reference plugin. */
+DCNV2_API dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const void* q,
+                                            const void* k, const int32_t* positions,
+                                            const float* freqs, const void* q_weight,
+                                            const void* k_weight, void* q_out, void* k_out,
+                                            dcnv2_stream_t stream);
+
+/* Attention of q_tokens queries to kv_tokens states of another sequence. Strides are in elements,
+ * in the order batch, token, head, multiples of 8; the elements of a head are contiguous. A batch
+ * or head stride of 0 in k and v shares those states. */
+typedef struct {
+  int32_t batch, q_tokens, kv_tokens;
+  int32_t q_heads, kv_heads;     /* q_heads a multiple of kv_heads: query head h reads kv head
+                                    h / (q_heads / kv_heads) */
+  int32_t head_dim;              /* a multiple of 8, at most 128 */
+  int32_t dtype;                 /* DCNV2_HALF or DCNV2_BF16: q, k, v and out */
+  float scale;                   /* of the scores, > 0 (usually 1 / sqrt(head_dim)) */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  int64_t mask_batch_stride;     /* bytes between the sequences of key_mask; 0: shared */
+} dcnv2_attention_desc;
+
+/* Workspace bytes of dcnv2_cross_attention (its error words). Returns 0 on a bad desc. */
+DCNV2_API size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc* desc);
+
+/* out = softmax(scale * q k^T over the kept keys) v, each query row over all kept states of its
+ * sequence. Tensor cores with fp32 accumulation and fp32 softmax statistics; the probabilities are
+ * rounded once to the inputs' type before the product with v.
+ *   kv_lens   int32 [batch] or NULL: states kept per sequence (values are clamped to
+ *             [0, kv_tokens]); NULL keeps kv_tokens.
+ *   key_mask  bytes [batch][kv_tokens] or NULL: state j is kept where the byte is not 0 (the pixels
+ *             of a padded image). Combined with kv_lens.
+ *   lse       fp32 [batch][q_heads][q_tokens] or NULL: natural logarithm of the sum of the exponentials.
+ * What states that are not kept hold (infinities, NaN) reaches no result. A sequence without any kept
+ * state gives zeros and lse = -inf. Deterministic: the same call gives the same bits. Pointers of
+ * q, k, v and out are 16-byte aligned device pointers of the current device; out overlaps no input.
+ * Asynchronous on `stream`; never allocates or synchronises. The workspace needs no setting up, and
+ * calls that may overlap on the GPU need one each. Single tokens and few rows split the states over
+ * a thread-block cluster. No counterpart in the reference plugin. */
+DCNV2_API dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void* q,
+                                             const void* k, const void* v,
+                                             const int32_t* kv_lens, const uint8_t* key_mask,
+                                             void* out, float* lse, void* workspace,
+                                             size_t workspace_bytes, dcnv2_stream_t stream);
+
+/* ORs the error words of the last dcnv2_cross_attention call with this desc and workspace into
+ * *code (0 = none, otherwise DCNV2_DEVERR_* bits, with DCNV2_ERR_DEVICE_TIMEOUT returned) after
+ * synchronising `stream`. Test and debug helper, not during a stream capture. */
+DCNV2_API dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
+                                                        const void* workspace,
+                                                        dcnv2_stream_t stream, int32_t* code);
 
 /* ---- Plugin object API (IPluginV3 + creator, without TensorRT types) ---- */
 

@@ -1,0 +1,330 @@
+// dcnv2_tokens.cu — host side of the token operators of include/dcnv2.h: argument checks, launch
+// shapes and the C entry points of dcnv2_qk_norm_rotary and dcnv2_cross_attention.
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/dcnv2.h"
+#include "dcnv2_attention_kernel.cuh"
+#include "dcnv2_host.cuh"
+#include "dcnv2_rotary_kernel.cuh"
+
+namespace dcnv2 {
+namespace {
+
+// The current device, or null when it cannot run this library's code.
+DevInfo* current_device(int* dev) {
+  if (cudaGetDevice(dev) != cudaSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  DevInfo* di = device_info(*dev);
+  return di && di->ok && di->major == 10 ? di : nullptr;
+}
+
+cudaLaunchConfig_t launch_config(unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
+                                 cudaLaunchAttribute (&attr)[2], unsigned cluster) {
+  // may start while the kernel ahead of it finishes; both kernels call griddep_wait before they
+  // touch memory
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cfg;
+}
+
+dcnv2_status launched(cudaError_t e) {
+  if (e == cudaSuccess) return DCNV2_OK;
+  cudaGetLastError();  // clear the launch error
+  return DCNV2_ERR_CUDA;
+}
+
+// ------------------------------------------------------------------ norm and rotation
+
+int rotary_elem_bytes(int dtype) {
+  return dtype == DCNV2_FLOAT ? 4 : dtype == DCNV2_HALF || dtype == DCNV2_BF16 ? 2 : 0;
+}
+
+// Whether `extent` steps of `stride` elements stay far inside 64 bits (and go forward).
+bool stride_ok(int64_t stride, int64_t extent) {
+  return stride >= 0 && (extent <= 1 || stride <= (int64_t(1) << 60) / extent);
+}
+
+dcnv2_status check_rotary(const dcnv2_rotary_desc* d) {
+  if (!d) return DCNV2_ERR_INVALID_ARG;
+  if (!rotary_elem_bytes(d->dtype)) return DCNV2_ERR_UNSUPPORTED;
+  if (d->batch < 0 || d->tokens < 0 || d->q_heads < 0 || d->k_heads < 0 ||
+      int64_t(d->q_heads) + d->k_heads < 1 || int64_t(d->q_heads) + d->k_heads > 65536)
+    return DCNV2_ERR_INVALID_ARG;
+  if (int64_t(d->batch) * d->tokens > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+  if (d->head_dim < 2 || d->head_dim % 2 || d->rotary_dim < 0 || d->rotary_dim % 2 ||
+      d->rotary_dim > d->head_dim)
+    return DCNV2_ERR_INVALID_ARG;
+  if (d->head_dim > 2 * kRotMaxPairs) return DCNV2_ERR_UNSUPPORTED;
+  if (d->norm != DCNV2_NORM_NONE && d->norm != DCNV2_NORM_RMS) return DCNV2_ERR_INVALID_ARG;
+  if (d->norm != DCNV2_NORM_NONE && !(d->eps >= 0.f && std::isfinite(d->eps)))
+    return DCNV2_ERR_INVALID_ARG;
+  if (d->interleaved != 0 && d->interleaved != 1) return DCNV2_ERR_INVALID_ARG;
+  if (d->rotary_dim > 0) {
+    if (d->axes < 1 || d->axes > 4) return DCNV2_ERR_INVALID_ARG;
+    for (int p = 0; p < d->rotary_dim / 2; ++p)
+      if (d->pair_axis[p] >= d->axes) return DCNV2_ERR_INVALID_ARG;
+    if (!stride_ok(d->pos_batch_stride, d->batch)) return DCNV2_ERR_INVALID_ARG;
+  }
+  const int64_t* in[2] = {d->q_stride, d->k_stride};
+  const int64_t* out[2] = {d->q_out_stride, d->k_out_stride};
+  const int heads[2] = {d->q_heads, d->k_heads};
+  for (int i = 0; i < 2; ++i) {
+    if (!heads[i]) continue;
+    const int64_t extent[3] = {d->batch, d->tokens, heads[i]};
+    for (int j = 0; j < 3; ++j) {
+      if (!stride_ok(in[i][j], extent[j]) || !stride_ok(out[i][j], extent[j]))
+        return DCNV2_ERR_INVALID_ARG;
+      // outputs of two rows at one place would race
+      if (extent[j] > 1 && out[i][j] < d->head_dim && d->batch && d->tokens)
+        return DCNV2_ERR_INVALID_ARG;
+    }
+  }
+  return DCNV2_OK;
+}
+
+// Pairs per chunk: the most of {16, 8 bytes, 1 element} that every address a lane forms allows
+// (pointers, strides and the places where the rotated pairs' halves and the rest begin).
+int rotary_vec(const dcnv2_rotary_desc& d, const RotaryArgs& a, int elem) {
+  const int rot = a.rot_pairs, rest = a.pairs - rot;
+  for (int bytes = 16; bytes >= 8; bytes >>= 1) {
+    const int vec = bytes / elem;
+    if (rot % vec || rest % vec) continue;
+    bool ok = true;
+    for (int i = 0; i < 2; ++i) {
+      const RotaryTensor& t = a.t[i];
+      if (!(i ? d.k_heads : d.q_heads)) continue;
+      const uintptr_t ptrs = reinterpret_cast<uintptr_t>(t.in) | reinterpret_cast<uintptr_t>(t.out) |
+                             reinterpret_cast<uintptr_t>(t.weight);
+      const int64_t strides = t.sb | t.st | t.sh | t.ob | t.ot | t.oh;
+      ok = ok && ptrs % bytes == 0 && strides % vec == 0;
+    }
+    if (ok) return vec;
+  }
+  return 1;
+}
+
+template <typename T, int VEC, int NC>
+dcnv2_status launch_rotary(const RotaryArgs& a, cudaStream_t st) {
+  cudaLaunchAttribute at[2];
+  const size_t smem = size_t(a.rows_per_block) * a.rot_pairs * sizeof(float2);
+  const cudaLaunchConfig_t cfg = launch_config(
+      static_cast<unsigned>(cdiv(a.rows, a.rows_per_block)), kRotThreads, smem, st, at, 1);
+  return launched(cudaLaunchKernelEx(&cfg, dcnv2_qk_norm_rotary_kernel<T, VEC, NC>, a));
+}
+
+// ------------------------------------------------------------------ attention
+
+struct AttnPlan {
+  unsigned grid = 0;
+};
+
+dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
+  if (!d) return DCNV2_ERR_INVALID_ARG;
+  if (d->dtype != DCNV2_HALF && d->dtype != DCNV2_BF16) return DCNV2_ERR_UNSUPPORTED;
+  if (d->batch < 0 || d->q_tokens < 0 || d->kv_tokens < 0 || d->q_heads < 1 || d->kv_heads < 1 ||
+      d->q_heads % d->kv_heads || d->head_dim < 1)
+    return DCNV2_ERR_INVALID_ARG;
+  if (d->head_dim % 8 || d->head_dim > 128) return DCNV2_ERR_UNSUPPORTED;
+  if (!(d->scale > 0.f && std::isfinite(d->scale))) return DCNV2_ERR_INVALID_ARG;
+  const int64_t qx[3] = {d->batch, d->q_tokens, d->q_heads};
+  const int64_t kx[3] = {d->batch, d->kv_tokens, d->kv_heads};
+  for (int j = 0; j < 3; ++j) {
+    if (!stride_ok(d->q_stride[j], qx[j]) || !stride_ok(d->out_stride[j], qx[j]) ||
+        !stride_ok(d->k_stride[j], kx[j]) || !stride_ok(d->v_stride[j], kx[j]))
+      return DCNV2_ERR_INVALID_ARG;
+    if (qx[j] > 1 && (d->q_stride[j] % 8 || d->out_stride[j] % 8)) return DCNV2_ERR_UNSUPPORTED;
+    if (kx[j] > 1 && (d->k_stride[j] % 8 || d->v_stride[j] % 8)) return DCNV2_ERR_UNSUPPORTED;
+    // outputs of two rows at one place would race
+    if (qx[j] > 1 && d->out_stride[j] < d->head_dim && d->batch && d->q_tokens)
+      return DCNV2_ERR_INVALID_ARG;
+  }
+  if (!stride_ok(d->mask_batch_stride, d->batch)) return DCNV2_ERR_INVALID_ARG;
+  const int64_t grid = cdiv(int64_t(d->batch) * d->q_tokens * d->q_heads, kAttnWarps);
+  if (grid >= INT_MAX) return DCNV2_ERR_INVALID_ARG;
+  p->grid = static_cast<unsigned>(grid);
+  return DCNV2_OK;
+}
+
+AttnTensor attn_tensor(const void* p, const int64_t (&stride)[3], int64_t batch, int64_t tokens,
+                       int64_t heads) {
+  // a stride that no second element is reached by may hold anything
+  return AttnTensor{p, batch > 1 ? stride[0] : 0, tokens > 1 ? stride[1] : 0,
+                    heads > 1 ? stride[2] : 0};
+}
+
+}  // namespace
+}  // namespace dcnv2
+
+using namespace dcnv2;
+
+extern "C" {
+
+dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const void* q, const void* k,
+                                  const int32_t* positions, const float* freqs,
+                                  const void* q_weight, const void* k_weight, void* q_out,
+                                  void* k_out, dcnv2_stream_t stream) {
+  const dcnv2_status s = check_rotary(desc);
+  if (s != DCNV2_OK) return s;
+  const dcnv2_rotary_desc& d = *desc;
+  if (d.batch == 0 || d.tokens == 0) return DCNV2_OK;
+  if ((d.q_heads && (!q || !q_out)) || (d.k_heads && (!k || !k_out)) ||
+      (d.rotary_dim && (!positions || !freqs)))
+    return DCNV2_ERR_INVALID_ARG;
+  const int elem = rotary_elem_bytes(d.dtype);
+  RotaryArgs a = {};
+  const bool norm = d.norm != DCNV2_NORM_NONE;
+  const void* in[2] = {q, k};
+  void* out[2] = {q_out, k_out};
+  const void* weight[2] = {norm ? q_weight : nullptr, norm ? k_weight : nullptr};
+  const int64_t* is[2] = {d.q_stride, d.k_stride};
+  const int64_t* os[2] = {d.q_out_stride, d.k_out_stride};
+  const int heads[2] = {d.q_heads, d.k_heads};
+  for (int i = 0; i < 2; ++i) {
+    if (!heads[i]) continue;
+    // a stride that no second element is reached by may hold anything
+    const bool many[3] = {d.batch > 1, d.tokens > 1, heads[i] > 1};
+    a.t[i] = RotaryTensor{in[i], out[i], weight[i],
+                          many[0] ? is[i][0] : 0, many[1] ? is[i][1] : 0, many[2] ? is[i][2] : 0,
+                          many[0] ? os[i][0] : 0, many[1] ? os[i][1] : 0, many[2] ? os[i][2] : 0};
+    if ((reinterpret_cast<uintptr_t>(in[i]) | reinterpret_cast<uintptr_t>(out[i]) |
+         reinterpret_cast<uintptr_t>(weight[i])) % elem)
+      return DCNV2_ERR_INVALID_ARG;
+  }
+  if ((reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(freqs)) % 4)
+    return DCNV2_ERR_INVALID_ARG;
+  a.pos = positions;
+  a.freqs = freqs;
+  a.pos_sb = d.batch > 1 ? d.pos_batch_stride : 0;
+  a.rows = d.batch * d.tokens;
+  a.tokens = d.tokens;
+  a.q_heads = d.q_heads;
+  a.heads = d.q_heads + d.k_heads;
+  a.D = d.head_dim;
+  a.pairs = d.head_dim / 2;
+  a.rot_pairs = d.rotary_dim / 2;
+  a.axes = d.axes;
+  a.norm = norm;
+  a.interleaved = d.interleaved;
+  a.eps = d.eps;
+  a.inv_d = 1.0f / static_cast<float>(d.head_dim);
+  for (int p = 0; p < a.rot_pairs; ++p)
+    a.pair_axis[p >> 4] |= static_cast<uint32_t>(d.pair_axis[p]) << (2 * (p & 15));
+  const int vec = rotary_vec(d, a, elem);
+  a.chunks = a.pairs / vec;
+  while ((1 << a.group_shift) < a.chunks && a.group_shift < 5) ++a.group_shift;
+  a.group = 1 << a.group_shift;
+  // Tokens per block: enough heads for every lane to have kRotBatch of them in flight, within
+  // 32 KB of cosines and sines.
+  const int64_t lanes = int64_t(a.heads) << a.group_shift;
+  int64_t rows = kRotThreads * kRotBatch / lanes;
+  const int64_t most = a.rot_pairs ? 32768 / (8 * a.rot_pairs) : 64;
+  rows = rows < most ? rows : most;
+  a.rows_per_block = static_cast<int>(rows < 1 ? 1 : rows);
+  int dev = 0;
+  if (!current_device(&dev)) return DCNV2_ERR_NO_DEVICE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (d.dtype == DCNV2_FLOAT)
+    return vec == 4   ? launch_rotary<float, 4, 1>(a, st)
+           : vec == 2 ? launch_rotary<float, 2, 2>(a, st)
+                      : launch_rotary<float, 1, 4>(a, st);
+  if (d.dtype == DCNV2_HALF)
+    return vec == 8   ? launch_rotary<__half, 8, 1>(a, st)
+           : vec == 4 ? launch_rotary<__half, 4, 1>(a, st)
+                      : launch_rotary<__half, 1, 4>(a, st);
+  return vec == 8   ? launch_rotary<__nv_bfloat16, 8, 1>(a, st)
+         : vec == 4 ? launch_rotary<__nv_bfloat16, 4, 1>(a, st)
+                    : launch_rotary<__nv_bfloat16, 1, 4>(a, st);
+}
+
+size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc* desc) {
+  AttnPlan p;
+  if (make_attn_plan(desc, &p) != DCNV2_OK) return 0;
+  return align_up(size_t(p.grid ? p.grid : 1) * sizeof(int), 256);
+}
+
+dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void* q, const void* k,
+                                   const void* v, const int32_t* kv_lens, const uint8_t* key_mask,
+                                   void* out, float* lse, void* workspace, size_t workspace_bytes,
+                                   dcnv2_stream_t stream) {
+  AttnPlan p;
+  const dcnv2_status s = make_attn_plan(desc, &p);
+  if (s != DCNV2_OK) return s;
+  const dcnv2_attention_desc& d = *desc;
+  if (d.batch == 0 || d.q_tokens == 0) return DCNV2_OK;
+  if (!q || !out || (d.kv_tokens && (!k || !v))) return DCNV2_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+       reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(out)) % 16)
+    return DCNV2_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(kv_lens) | reinterpret_cast<uintptr_t>(lse)) % 4)
+    return DCNV2_ERR_INVALID_ARG;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 ||
+      workspace_bytes < size_t(p.grid) * sizeof(int))
+    return DCNV2_ERR_WORKSPACE;
+  int dev = 0;
+  DevInfo* di = current_device(&dev);
+  if (!di) return DCNV2_ERR_NO_DEVICE;
+  AttnArgs a = {};
+  a.q = attn_tensor(q, d.q_stride, d.batch, d.q_tokens, d.q_heads);
+  a.o = attn_tensor(out, d.out_stride, d.batch, d.q_tokens, d.q_heads);
+  a.k = attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads);
+  a.v = attn_tensor(v, d.v_stride, d.batch, d.kv_tokens, d.kv_heads);
+  a.kv_lens = kv_lens;
+  a.key_mask = key_mask;
+  a.mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
+  a.lse = lse;
+  a.err = static_cast<int*>(workspace);
+  a.B = d.batch; a.L = d.q_tokens; a.S = d.kv_tokens;
+  a.H = d.q_heads; a.G = d.kv_heads; a.D = d.head_dim;
+  a.scale = d.scale;
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg = launch_config(p.grid, kAttnWarps * 32, 0,
+                                               reinterpret_cast<cudaStream_t>(stream), at, 1);
+  return launched(d.dtype == DCNV2_HALF
+                      ? cudaLaunchKernelEx(&cfg, dcnv2_cross_attention_kernel<__half>, a)
+                      : cudaLaunchKernelEx(&cfg, dcnv2_cross_attention_kernel<__nv_bfloat16>, a));
+}
+
+dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
+                                              const void* workspace, dcnv2_stream_t stream,
+                                              int32_t* code) {
+  AttnPlan p;
+  const dcnv2_status s = make_attn_plan(desc, &p);
+  if (s != DCNV2_OK) return s;
+  if (!workspace || !code) return DCNV2_ERR_INVALID_ARG;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int32_t bits = 0;
+  const int* words = static_cast<const int*>(workspace);
+  for (unsigned at = 0; at < p.grid;) {
+    int32_t part[1024];
+    const unsigned n = p.grid - at < 1024u ? p.grid - at : 1024u;
+    if (cudaMemcpyAsync(part, words + at, n * sizeof(int), cudaMemcpyDeviceToHost, st) !=
+            cudaSuccess ||
+        cudaStreamSynchronize(st) != cudaSuccess) {
+      cudaGetLastError();
+      return DCNV2_ERR_CUDA;
+    }
+    for (unsigned i = 0; i < n; ++i) bits |= part[i];
+    at += n;
+  }
+  *code = bits;
+  return bits ? DCNV2_ERR_DEVICE_TIMEOUT : DCNV2_OK;
+}
+
+}  // extern "C"

@@ -37,6 +37,7 @@ class DType(enum.IntEnum):
     FLOAT = 0
     HALF = 1
     INT8 = 2
+    BF16 = 7   # token operators only
 
 
 class Math(enum.IntEnum):
@@ -54,6 +55,28 @@ class Desc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in (
         "n", "c", "h", "w", "out_c", "kernel", "stride", "padding", "dilation",
         "deformable_groups", "dtype", "math")]
+
+
+class Norm(enum.IntEnum):
+    """Norms of dcnv2_qk_norm_rotary."""
+    NONE = 0
+    RMS = 1
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "tokens", "q_heads", "k_heads", "head_dim", "rotary_dim", "axes", "dtype", "norm",
+        "interleaved")] + [("eps", ctypes.c_float), ("pair_axis", ctypes.c_uint8 * 128)] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride",
+                                          "k_out_stride")] + [("pos_batch_stride", ctypes.c_int64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "batch", "q_tokens", "kv_tokens", "q_heads", "kv_heads", "head_dim", "dtype")] + [
+        ("scale", ctypes.c_float)] + [(n, ctypes.c_int64 * 3) for n in (
+            "q_stride", "k_stride", "v_stride", "out_stride")] + [
+        ("mask_batch_stride", ctypes.c_int64)]
 
 
 class TensorDesc(ctypes.Structure):
@@ -91,6 +114,12 @@ def _load() -> ctypes.CDLL:
         "dcnv2_forward_host_workspace_size": (ctypes.c_size_t, [Dp, ctypes.c_int32]),
         "dcnv2_forward_host": (ctypes.c_int, [Dp, P, P, P, P, P, P, P, ctypes.c_size_t,
                                               ctypes.c_float, ctypes.c_float, ctypes.c_int32, P]),
+        "dcnv2_qk_norm_rotary": (ctypes.c_int, [ctypes.POINTER(RotaryDesc)] + [P] * 9),
+        "dcnv2_cross_attention_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(AttentionDesc)]),
+        "dcnv2_cross_attention": (ctypes.c_int, [ctypes.POINTER(AttentionDesc)] + [P] * 8 +
+                                  [ctypes.c_size_t, P]),
+        "dcnv2_cross_attention_read_error": (ctypes.c_int, [
+            ctypes.POINTER(AttentionDesc), P, P, ctypes.POINTER(ctypes.c_int32)]),
         "dcnv2_uses_tensor_cores": (ctypes.c_int32, [Dp]),
         "dcnv2_launch_count": (ctypes.c_int32, [Dp]),
         "dcnv2_diag_main_kernel": (ctypes.c_char_p, [Dp]),
@@ -155,6 +184,8 @@ EXPORTED = (
     "dcnv2_forward_static_scratch", "dcnv2_read_static_scratch_error", "dcnv2_read_device_error",
     "dcnv2_forward_with_head_workspace_size", "dcnv2_forward_with_head",
     "dcnv2_forward_host_workspace_size", "dcnv2_forward_host",
+    "dcnv2_qk_norm_rotary", "dcnv2_cross_attention_workspace_size", "dcnv2_cross_attention",
+    "dcnv2_cross_attention_read_error",
     "dcnv2_uses_tensor_cores", "dcnv2_launch_count", "dcnv2_status_string", "dcnv2_plugin_name",
     "dcnv2_plugin_version", "dcnv2_plugin_namespace", "dcnv2_plugin_field_names",
     "dcnv2_plugin_create", "dcnv2_plugin_clone", "dcnv2_plugin_destroy",
@@ -303,3 +334,17 @@ def forward_with_head_raw(desc: Desc, x, head_weight, head_bias, weight, bias, y
     return int(lib.dcnv2_forward_with_head(ctypes.byref(desc), x, head_weight, head_bias, weight,
                                            bias, y, offset_out, mask_out, workspace,
                                            workspace_bytes, stream))
+
+
+def attention_workspace_size(desc: AttentionDesc) -> int:
+    return int(lib.dcnv2_cross_attention_workspace_size(ctypes.byref(desc)))
+
+
+def cross_attention_error(desc: AttentionDesc, workspace, stream=0) -> int:
+    """Error bits of the last dcnv2_cross_attention call with this desc and workspace address."""
+    code = ctypes.c_int32(0)
+    st = lib.dcnv2_cross_attention_read_error(ctypes.byref(desc), workspace, stream,
+                                              ctypes.byref(code))
+    if st not in (Status.OK, Status.ERR_DEVICE_TIMEOUT):
+        raise DCNv2Error(st, "dcnv2_cross_attention_read_error")
+    return int(code.value)
