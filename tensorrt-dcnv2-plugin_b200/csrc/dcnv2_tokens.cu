@@ -132,8 +132,14 @@ dcnv2_status launch_rotary(const RotaryArgs& a, cudaStream_t st) {
 // ------------------------------------------------------------------ attention
 
 struct AttnPlan {
+  bool paired = false;     // one tile of rows, the warpgroups alternate over the states
+  bool wide = false;       // heads of more than 64 elements
+  int row_tiles = 0, split = 1;
   unsigned grid = 0;
 };
+
+constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
+constexpr int kAttnMaxSplit = 8;  // portable cluster size
 
 dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   if (!d) return DCNV2_ERR_INVALID_ARG;
@@ -156,9 +162,19 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
       return DCNV2_ERR_INVALID_ARG;
   }
   if (!stride_ok(d->mask_batch_stride, d->batch)) return DCNV2_ERR_INVALID_ARG;
-  const int64_t grid = cdiv(int64_t(d->batch) * d->q_tokens * d->q_heads, kAttnWarps);
-  if (grid >= INT_MAX) return DCNV2_ERR_INVALID_ARG;
-  p->grid = static_cast<unsigned>(grid);
+  p->wide = d->head_dim > 64;
+  const int64_t rows = int64_t(d->q_tokens) * (d->q_heads / d->kv_heads);
+  if (rows > INT_MAX - 2 * kAttnTile) return DCNV2_ERR_INVALID_ARG;
+  p->paired = rows <= kAttnTile;
+  p->row_tiles = static_cast<int>(cdiv(rows, p->paired ? kAttnTile : 2 * kAttnTile));
+  const int64_t ctas = int64_t(d->batch) * d->kv_heads * p->row_tiles;
+  // Split the states over as many CTAs as still run at once, each with a tile at least.
+  p->split = 1;
+  while (p->split < kAttnMaxSplit && ctas * p->split * 2 <= kPlanSms &&
+         cdiv(d->kv_tokens, kAttnTile) >= int64_t(p->split) * 2 * (p->paired ? 2 : 1))
+    p->split *= 2;
+  if (ctas * p->split > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+  p->grid = static_cast<unsigned>(ctas * p->split);
   return DCNV2_OK;
 }
 
@@ -167,6 +183,61 @@ AttnTensor attn_tensor(const void* p, const int64_t (&stride)[3], int64_t batch,
   // a stride that no second element is reached by may hold anything
   return AttnTensor{p, batch > 1 ? stride[0] : 0, tokens > 1 ? stride[1] : 0,
                     heads > 1 ? stride[2] : 0};
+}
+
+// Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x 128 tokens in the
+// 128-byte swizzle. Axes that no step is taken along, or that share their states, have extent 1.
+// What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
+bool attn_tensor_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
+                     const dcnv2_attention_desc& d, int* batch_step, int* head_step) {
+  const bool heads = d.kv_heads > 1 && stride[2] > 0, batch = d.batch > 1 && stride[0] > 0;
+  *head_step = heads;
+  *batch_step = batch;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d.head_dim),
+                              static_cast<cuuint64_t>(d.kv_tokens),
+                              static_cast<cuuint64_t>(heads ? d.kv_heads : 1),
+                              static_cast<cuuint64_t>(batch ? d.batch : 1)};
+  const cuuint64_t row = static_cast<cuuint64_t>(d.head_dim) * 2;
+  const cuuint64_t strides[3] = {d.kv_tokens > 1 ? static_cast<cuuint64_t>(stride[1]) * 2 : row,
+                                 heads ? static_cast<cuuint64_t>(stride[2]) * 2 : row,
+                                 batch ? static_cast<cuuint64_t>(stride[0]) * 2 : row};
+  const cuuint32_t box[4] = {64, kAttnTile, 1, 1}, ones[4] = {1, 1, 1, 1};
+  std::memset(m, 0, sizeof(*m));
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  return encode &&
+         encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(p), dims, strides, box, ones,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, bool PAIRED, bool BF16>
+dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
+                              const AttnPlan& p, int dev, cudaStream_t st) {
+  auto kernel = dcnv2_cross_attention_kernel<DP, PAIRED, BF16>;
+  constexpr size_t smem = attn_smem_bytes<DP, PAIRED>();
+  static_assert(smem <= kSmemLimit, "shared memory");
+  static std::atomic<bool> set[kMaxDevices];  // per device; setting it twice does no harm
+  if (!set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return launched(e);
+    set[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg =
+      launch_config(p.grid, kAttnThreads, smem, st, at, static_cast<unsigned>(p.split));
+  return launched(cudaLaunchKernelEx(&cfg, kernel, a, mk, mv));
+}
+
+template <bool BF16>
+dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
+                              const AttnPlan& p, int dev, cudaStream_t st) {
+  if (p.wide)
+    return p.paired ? launch_attention<128, true, BF16>(a, mk, mv, p, dev, st)
+                    : launch_attention<128, false, BF16>(a, mk, mv, p, dev, st);
+  return p.paired ? launch_attention<64, true, BF16>(a, mk, mv, p, dev, st)
+                  : launch_attention<64, false, BF16>(a, mk, mv, p, dev, st);
 }
 
 }  // namespace
@@ -283,22 +354,29 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
   AttnArgs a = {};
   a.q = attn_tensor(q, d.q_stride, d.batch, d.q_tokens, d.q_heads);
   a.o = attn_tensor(out, d.out_stride, d.batch, d.q_tokens, d.q_heads);
-  a.k = attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads);
-  a.v = attn_tensor(v, d.v_stride, d.batch, d.kv_tokens, d.kv_heads);
   a.kv_lens = kv_lens;
   a.key_mask = key_mask;
   a.mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
   a.lse = lse;
   a.err = static_cast<int*>(workspace);
-  a.B = d.batch; a.L = d.q_tokens; a.S = d.kv_tokens;
-  a.H = d.q_heads; a.G = d.kv_heads; a.D = d.head_dim;
+  a.L = d.q_tokens; a.S = d.kv_tokens; a.H = d.q_heads; a.G = d.kv_heads; a.D = d.head_dim;
+  a.group = d.q_heads / d.kv_heads;
+  a.rows = d.q_tokens * a.group;
+  a.row_tiles = p.row_tiles;
+  a.split = p.split;
   a.scale = d.scale;
-  cudaLaunchAttribute at[2];
-  const cudaLaunchConfig_t cfg = launch_config(p.grid, kAttnWarps * 32, 0,
-                                               reinterpret_cast<cudaStream_t>(stream), at, 1);
-  return launched(d.dtype == DCNV2_HALF
-                      ? cudaLaunchKernelEx(&cfg, dcnv2_cross_attention_kernel<__half>, a)
-                      : cudaLaunchKernelEx(&cfg, dcnv2_cross_attention_kernel<__nv_bfloat16>, a));
+  a.timeout_ns = kDefaultTimeoutNs;
+  CUtensorMap mk, mv;
+  if (d.kv_tokens == 0) {  // nothing is loaded
+    std::memset(&mk, 0, sizeof(mk));
+    mv = mk;
+  } else if (!attn_tensor_map(&mk, k, d.k_stride, d, &a.k_batch, &a.k_head) ||
+             !attn_tensor_map(&mv, v, d.v_stride, d, &a.v_batch, &a.v_head)) {
+    return DCNV2_ERR_UNSUPPORTED;  // strides of 2^40 bytes and more
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return d.dtype == DCNV2_BF16 ? launch_attention<true>(a, mk, mv, p, dev, st)
+                               : launch_attention<false>(a, mk, mv, p, dev, st);
 }
 
 dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/dcnv2.h"
 #include "ptx_sm100.cuh"
 
 namespace dcnv2 {
@@ -42,6 +43,20 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Wa
         atomicOr(w.err, code);
         return false;
       }
+    }
+  }
+}
+
+// The same wait for what a kernel itself still has in flight (copies, MMAs) before it ends or frees
+// tensor memory: an abort does not cut it short, only the time limit does.
+__device__ __forceinline__ bool drain_bar(uint32_t bar, uint32_t parity, const WaitCtx& w) {
+  const uint64_t t0 = ptx::global_timer_ns();
+  for (;;) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if (ptx::global_timer_ns() - t0 > w.timeout_ns) {
+      *w.abort_flag = 1;
+      atomicOr(w.err, DCNV2_DEVERR_TIMEOUT_DRAIN);
+      return false;
     }
   }
 }
