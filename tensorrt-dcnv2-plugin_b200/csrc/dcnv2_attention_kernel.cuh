@@ -253,89 +253,100 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp == kAttnMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
-      const uint32_t id_s = ptx::make_idesc(1, fmt, kAttnTile);
-      const uint32_t n_o = static_cast<uint32_t>((args.D + 15) / 16 * 16);
-      const uint32_t id_o = ptx::make_idesc(1, fmt, n_o) | ptx::kIdescBMn;
-      const int d_steps = (args.D + 15) / 16;
-      bool ok = wait_bar(q_full, 0, wc, DCNV2_DEVERR_TIMEOUT_MMA);
-      // whether tile i exists (its words are there), or the states have ended
-      auto exists = [&](int i) {
-        ok = ok && wait_bar(info_full + 8 * (i % NI), static_cast<uint32_t>(i / NI) & 1u, wc,
-                            DCNV2_DEVERR_TIMEOUT_MMA);
-        return ok && ptx::ld_shared_u32_volatile(base + LY::kInfo + (i % NI) * 32 + 16) == 0;
-      };
-      auto scores = [&](int i, int wg) {  // S of warpgroup wg from K tile i
-        const uint32_t q = base + LY::kQ + (PAIRED ? 0 : wg) * LY::kTileBytes;
-        const uint32_t k = base + LY::kK + (i % NS) * LY::kTileBytes;
-        for (int x = 0; x < d_steps; ++x) {
-          const uint32_t off = (x >> 2) * kAttnBlockBytes + (x & 3) * 32;
-          ptx::mma_f16(tmem + kAttnTile * wg, ptx::sw128_kmajor_desc(q + off),
-                       ptx::sw128_kmajor_desc(k + off), id_s, x > 0);
+    // The warp runs this code as a whole (descriptors and barrier addresses stay in uniform
+    // registers); one elected lane issues.
+    constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
+    const uint32_t id_s = ptx::make_idesc(1, fmt, kAttnTile);
+    const uint32_t id_o =
+        ptx::make_idesc(1, fmt, static_cast<uint32_t>((args.D + 15) / 16 * 16)) | ptx::kIdescBMn;
+    const int d_steps = (args.D + 15) / 16;
+    const bool leader = ptx::elect_one();
+    const uint64_t q_desc = ptx::sw128_kmajor_desc(base + LY::kQ);
+    const uint64_t k_desc = ptx::sw128_kmajor_desc(base + LY::kK);
+    const uint64_t v_desc = ptx::sw128_mnmajor_desc(base + LY::kV, kAttnBlockBytes);
+    bool ok = wait_bar(q_full, 0, wc, DCNV2_DEVERR_TIMEOUT_MMA);
+    // whether tile i exists (its words are there), or the states have ended
+    auto exists = [&](int i) {
+      ok = ok && wait_bar(info_full + 8 * (i % NI), static_cast<uint32_t>(i / NI) & 1u, wc,
+                          DCNV2_DEVERR_TIMEOUT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+      return ok && ptx::ld_shared_u32_volatile(base + LY::kInfo + (i % NI) * 32 + 16) == 0;
+    };
+    auto commit = [&](uint32_t bar) {
+      if (leader) ptx::tc_commit(bar);
+    };
+    auto scores = [&](int i, int wg) {  // S of warpgroup wg from K tile i
+      const uint64_t q = q_desc + (PAIRED ? 0 : wg) * (LY::kTileBytes >> 4);
+      const uint64_t k = k_desc + (i % NS) * (LY::kTileBytes >> 4);
+      const uint32_t d = tmem + kAttnTile * wg;
+      if (leader) {
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          const uint32_t off = ((x >> 2) * kAttnBlockBytes + (x & 3) * 32) >> 4;
+          if (x < d_steps) ptx::mma_f16(d, q + off, k + off, id_s, x > 0);
         }
         ptx::tc_commit(s_full + 8 * wg);
-      };
-      auto product = [&](int i, int wg, bool first) {  // O of warpgroup wg += P V tile i
-        const uint64_t v = ptx::sw128_mnmajor_desc(base + LY::kV + (i % NS) * LY::kTileBytes,
-                                                   kAttnBlockBytes);
+      }
+    };
+    auto product = [&](int i, int wg, bool first) {  // O of warpgroup wg += P V tile i
+      const uint64_t v = v_desc + (i % NS) * (LY::kTileBytes >> 4);
+      const uint32_t d = tmem + 2 * kAttnTile + DP * wg, p = tmem + kAttnTile * wg;
+      if (leader) {
 #pragma unroll
         for (int x = 0; x < kAttnTile / 16; ++x)
-          ptx::mma_f16_ta(tmem + 2 * kAttnTile + DP * wg, tmem + kAttnTile * wg + 8 * x,
-                          v + x * (2048 >> 4), id_o, !first || x > 0);
-      };
-      auto wait_k = [&](int i) {
-        ok = ok && wait_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc,
-                            DCNV2_DEVERR_TIMEOUT_MMA);
-        ptx::tc_fence_after();
-        return ok;
-      };
-      auto wait_pv = [&](int i, int wg, uint32_t turn) {
-        ok = ok && wait_bar(v_ready + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc,
-                            DCNV2_DEVERR_TIMEOUT_MMA) &&
-             wait_bar(p_ready + 8 * wg, turn & 1u, wc, DCNV2_DEVERR_TIMEOUT_MMA);
-        ptx::tc_fence_after();
-        return ok;
-      };
-      // A warpgroup's next scores are issued right behind its product, whose probabilities they
-      // overwrite: the tensor core runs MMAs in the order of issue.
-      if (PAIRED) {
-        for (int i = 0; i < 2; ++i)
-          if (exists(i) && wait_k(i)) {
-            scores(i, i);
-            ptx::tc_commit(k_empty + 8 * (i % NS));
-          }
-        for (int i = 0; ok && exists(i); ++i) {
-          const int wg = i & 1;
-          if (!wait_pv(i, wg, static_cast<uint32_t>(i >> 1))) break;
-          product(i, wg, i < 2);
-          ptx::tc_commit(v_empty + 8 * (i % NS));
-          // the second end mark stands at most two behind the last tile
-          if (!exists(i + 1)) continue;
-          if (exists(i + 2) && wait_k(i + 2)) {
-            scores(i + 2, wg);
-            ptx::tc_commit(k_empty + 8 * ((i + 2) % NS));
-          }
+          ptx::mma_f16_ta(d, p + 8 * x, v + x * (2048 >> 4), id_o, !first || x > 0);
+      }
+    };
+    auto wait_k = [&](int i) {
+      ok = ok && wait_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc,
+                          DCNV2_DEVERR_TIMEOUT_MMA);
+      ptx::tc_fence_after();
+      return ok = __all_sync(0xffffffffu, ok);
+    };
+    auto wait_pv = [&](int i, int wg, uint32_t turn) {
+      ok = ok && wait_bar(v_ready + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc,
+                          DCNV2_DEVERR_TIMEOUT_MMA) &&
+           wait_bar(p_ready + 8 * wg, turn & 1u, wc, DCNV2_DEVERR_TIMEOUT_MMA);
+      ptx::tc_fence_after();
+      return ok = __all_sync(0xffffffffu, ok);
+    };
+    // A warpgroup's next scores are issued right behind its product, whose probabilities they
+    // overwrite: the tensor core runs MMAs in the order of issue.
+    if (PAIRED) {
+      for (int i = 0; i < 2; ++i)
+        if (exists(i) && wait_k(i)) {
+          scores(i, i);
+          commit(k_empty + 8 * (i % NS));
         }
-      } else if (exists(0) && wait_k(0)) {
-        scores(0, 0);
-        scores(0, 1);
-        ptx::tc_commit(k_empty);
-        for (int i = 0;; ++i) {
-          const bool more = exists(i + 1);
-          for (int wg = 0; wg < 2 && ok; ++wg) {
-            if (!wait_pv(i, wg, static_cast<uint32_t>(i))) break;
-            product(i, wg, i == 0);
-            if (wg) ptx::tc_commit(v_empty + 8 * (i % NS));
-            if (more && wait_k(i + 1)) scores(i + 1, wg);
-          }
-          if (!more || !ok) break;
-          ptx::tc_commit(k_empty + 8 * ((i + 1) % NS));
+      for (int i = 0; ok && exists(i); ++i) {
+        const int wg = i & 1;
+        if (!wait_pv(i, wg, static_cast<uint32_t>(i >> 1))) break;
+        product(i, wg, i < 2);
+        commit(v_empty + 8 * (i % NS));
+        // the second end mark stands at most two behind the last tile
+        if (exists(i + 1) && exists(i + 2) && wait_k(i + 2)) {
+          scores(i + 2, wg);
+          commit(k_empty + 8 * ((i + 2) % NS));
         }
       }
-      ptx::tc_commit(o_final);
-      drain_bar(o_final, 0, wc);
+    } else if (exists(0) && wait_k(0)) {
+      scores(0, 0);
+      scores(0, 1);
+      commit(k_empty);
+      for (int i = 0;; ++i) {
+        const bool more = exists(i + 1);
+        for (int wg = 0; wg < 2 && ok; ++wg) {
+          if (!wait_pv(i, wg, static_cast<uint32_t>(i))) break;
+          product(i, wg, i == 0);
+          if (wg) commit(v_empty + 8 * (i % NS));
+          if (more && wait_k(i + 1)) scores(i + 1, wg);
+        }
+        if (!more || !ok) break;
+        commit(k_empty + 8 * ((i + 1) % NS));
+      }
     }
+    commit(o_final);
+    drain_bar(o_final, 0, wc);
   } else if (warp == kAttnFixWarp) {
     // ------------------------------------------------------------ V rows of unkept states
     for (int i = 0;; ++i) {
