@@ -120,13 +120,41 @@ int rotary_vec(const dcnv2_rotary_desc& d, const RotaryArgs& a, int elem) {
   return 1;
 }
 
-template <typename T, int VEC, int NC>
-dcnv2_status launch_rotary(const RotaryArgs& a, cudaStream_t st) {
+template <typename T, int VEC, int NC, bool INTER>
+dcnv2_status launch_rotary(RotaryArgs a, const DevInfo& di, cudaStream_t st) {
+  const int64_t most = int64_t(di.sm_count) * kRotResident;  // warps
+  int64_t units = 0;
+  for (int i = 0; i < 2; ++i) {
+    if (!a.heads[i]) continue;
+    // heads side by side: a power of two, within the warp, and enough lanes to keep the cosines
+    int& sh = a.side_shift[i];
+    while (sh + a.group_shift < 5 && ((kRotHeads << sh) < a.heads[i] ||
+                                      2 * a.rot_pairs > (kRotLane << (sh + a.group_shift))))
+      ++sh;
+    const int64_t blocks = cdiv(a.rows, 32 >> (sh + a.group_shift));
+    const int all_steps = static_cast<int>(cdiv(a.heads[i], int64_t(kRotHeads) << sh));
+    // all heads of a token in one unit, unless that leaves warps without work
+    const int64_t want = cdiv(most, blocks);
+    a.steps[i] = static_cast<int>(cdiv(all_steps, want < all_steps ? want : all_steps));
+    a.parts[i] = static_cast<int>(cdiv(all_steps, a.steps[i]));
+    if (blocks * a.parts[i] > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+    a.units[i] = static_cast<int>(blocks * a.parts[i]);
+    units += a.units[i];
+  }
+  const int64_t grid = cdiv(units < most ? units : most, kRotWarps);
   cudaLaunchAttribute at[2];
-  const size_t smem = size_t(a.rows_per_block) * a.rot_pairs * sizeof(float2);
-  const cudaLaunchConfig_t cfg = launch_config(
-      static_cast<unsigned>(cdiv(a.rows, a.rows_per_block)), kRotThreads, smem, st, at, 1);
-  return launched(cudaLaunchKernelEx(&cfg, dcnv2_qk_norm_rotary_kernel<T, VEC, NC>, a));
+  const size_t smem = kRotMaxPairs * (sizeof(uint64_t) + sizeof(int)) +
+                      size_t(kRotThreads) * kRotLane * sizeof(float);
+  const cudaLaunchConfig_t cfg =
+      launch_config(static_cast<unsigned>(grid), kRotThreads, smem, st, at, 1);
+  return launched(cudaLaunchKernelEx(&cfg, dcnv2_qk_norm_rotary_kernel<T, VEC, NC, INTER>, a));
+}
+
+template <typename T, int VEC, int NC>
+dcnv2_status launch_rotary(const RotaryArgs& a, bool interleaved, const DevInfo& di,
+                           cudaStream_t st) {
+  return interleaved ? launch_rotary<T, VEC, NC, true>(a, di, st)
+                     : launch_rotary<T, VEC, NC, false>(a, di, st);
 }
 
 // ------------------------------------------------------------------ attention
@@ -285,14 +313,12 @@ dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const void* q, 
   a.pos_sb = d.batch > 1 ? d.pos_batch_stride : 0;
   a.rows = d.batch * d.tokens;
   a.tokens = d.tokens;
-  a.q_heads = d.q_heads;
-  a.heads = d.q_heads + d.k_heads;
-  a.D = d.head_dim;
+  a.heads[0] = d.q_heads;
+  a.heads[1] = d.k_heads;
   a.pairs = d.head_dim / 2;
   a.rot_pairs = d.rotary_dim / 2;
   a.axes = d.axes;
   a.norm = norm;
-  a.interleaved = d.interleaved;
   a.eps = d.eps;
   a.inv_d = 1.0f / static_cast<float>(d.head_dim);
   for (int p = 0; p < a.rot_pairs; ++p)
@@ -300,28 +326,22 @@ dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const void* q, 
   const int vec = rotary_vec(d, a, elem);
   a.chunks = a.pairs / vec;
   while ((1 << a.group_shift) < a.chunks && a.group_shift < 5) ++a.group_shift;
-  a.group = 1 << a.group_shift;
-  // Tokens per block: enough heads for every lane to have kRotBatch of them in flight, within
-  // 32 KB of cosines and sines.
-  const int64_t lanes = int64_t(a.heads) << a.group_shift;
-  int64_t rows = kRotThreads * kRotBatch / lanes;
-  const int64_t most = a.rot_pairs ? 32768 / (8 * a.rot_pairs) : 64;
-  rows = rows < most ? rows : most;
-  a.rows_per_block = static_cast<int>(rows < 1 ? 1 : rows);
   int dev = 0;
-  if (!current_device(&dev)) return DCNV2_ERR_NO_DEVICE;
+  const DevInfo* di = current_device(&dev);
+  if (!di) return DCNV2_ERR_NO_DEVICE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const bool inter = d.interleaved != 0;
   if (d.dtype == DCNV2_FLOAT)
-    return vec == 4   ? launch_rotary<float, 4, 1>(a, st)
-           : vec == 2 ? launch_rotary<float, 2, 2>(a, st)
-                      : launch_rotary<float, 1, 4>(a, st);
+    return vec == 4   ? launch_rotary<float, 4, 1>(a, inter, *di, st)
+           : vec == 2 ? launch_rotary<float, 2, 2>(a, inter, *di, st)
+                      : launch_rotary<float, 1, 4>(a, inter, *di, st);
   if (d.dtype == DCNV2_HALF)
-    return vec == 8   ? launch_rotary<__half, 8, 1>(a, st)
-           : vec == 4 ? launch_rotary<__half, 4, 1>(a, st)
-                      : launch_rotary<__half, 1, 4>(a, st);
-  return vec == 8   ? launch_rotary<__nv_bfloat16, 8, 1>(a, st)
-         : vec == 4 ? launch_rotary<__nv_bfloat16, 4, 1>(a, st)
-                    : launch_rotary<__nv_bfloat16, 1, 4>(a, st);
+    return vec == 8   ? launch_rotary<__half, 8, 1>(a, inter, *di, st)
+           : vec == 4 ? launch_rotary<__half, 4, 1>(a, inter, *di, st)
+                      : launch_rotary<__half, 1, 4>(a, inter, *di, st);
+  return vec == 8   ? launch_rotary<__nv_bfloat16, 8, 1>(a, inter, *di, st)
+         : vec == 4 ? launch_rotary<__nv_bfloat16, 4, 1>(a, inter, *di, st)
+                    : launch_rotary<__nv_bfloat16, 1, 4>(a, inter, *di, st);
 }
 
 size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc* desc) {
