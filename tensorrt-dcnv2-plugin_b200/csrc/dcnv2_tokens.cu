@@ -8,6 +8,7 @@
 
 #include "../../include/dcnv2.h"
 #include "dcnv2_attention_kernel.cuh"
+#include "dcnv2_attention_step_kernel.cuh"
 #include "dcnv2_host.cuh"
 #include "dcnv2_rotary_kernel.cuh"
 
@@ -160,6 +161,7 @@ dcnv2_status launch_rotary(const RotaryArgs& a, bool interleaved, const DevInfo&
 // ------------------------------------------------------------------ attention
 
 struct AttnPlan {
+  bool step = false;       // few rows: dcnv2_attention_step_kernel
   bool paired = false;     // one tile of rows, the warpgroups alternate over the states
   bool wide = false;       // heads of more than 64 elements
   int row_tiles = 0, split = 1;
@@ -193,6 +195,18 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   p->wide = d->head_dim > 64;
   const int64_t rows = int64_t(d->q_tokens) * (d->q_heads / d->kv_heads);
   if (rows > INT_MAX - 2 * kAttnTile) return DCNV2_ERR_INVALID_ARG;
+  p->step = rows <= kStepRows;
+  if (p->step) {
+    const int64_t units = int64_t(d->batch) * d->kv_heads;
+    const int keys = d->head_dim > 64 ? 16 : d->head_dim > 32 ? 32 : 64;
+    p->split = 1;
+    while (p->split < kAttnMaxSplit && units * p->split < 4 * kPlanSms &&
+           cdiv(d->kv_tokens, keys) >= int64_t(p->split) * 2 * kStepWarps * 2)
+      p->split *= 2;
+    if (units * p->split > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+    p->grid = static_cast<unsigned>(units * p->split);
+    return DCNV2_OK;
+  }
   p->paired = rows <= kAttnTile;
   p->row_tiles = static_cast<int>(cdiv(rows, p->paired ? kAttnTile : 2 * kAttnTile));
   const int64_t ctas = int64_t(d->batch) * d->kv_heads * p->row_tiles;
@@ -266,6 +280,30 @@ dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CU
                     : launch_attention<128, false, BF16>(a, mk, mv, p, dev, st);
   return p.paired ? launch_attention<64, true, BF16>(a, mk, mv, p, dev, st)
                   : launch_attention<64, false, BF16>(a, mk, mv, p, dev, st);
+}
+
+template <int DP, bool BF16>
+dcnv2_status launch_step(const AttnStepArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+  auto kernel = dcnv2_attention_step_kernel<DP, BF16>;
+  constexpr size_t smem = StepLayout<DP>::kTotal;
+  static std::atomic<bool> set[kMaxDevices];  // per device; setting it twice does no harm
+  if (!set[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(smem));
+    if (e != cudaSuccess) return launched(e);
+    set[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchAttribute at[2];
+  const cudaLaunchConfig_t cfg =
+      launch_config(p.grid, kStepThreads, smem, st, at, static_cast<unsigned>(p.split));
+  return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
+template <bool BF16>
+dcnv2_status launch_step(const AttnStepArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+  return a.D > 64   ? launch_step<128, BF16>(a, p, dev, st)
+         : a.D > 32 ? launch_step<64, BF16>(a, p, dev, st)
+                    : launch_step<32, BF16>(a, p, dev, st);
 }
 
 }  // namespace
@@ -371,17 +409,33 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
   int dev = 0;
   DevInfo* di = current_device(&dev);
   if (!di) return DCNV2_ERR_NO_DEVICE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int group = d.q_heads / d.kv_heads;
+  const AttnTensor tq = attn_tensor(q, d.q_stride, d.batch, d.q_tokens, d.q_heads);
+  const AttnTensor to = attn_tensor(out, d.out_stride, d.batch, d.q_tokens, d.q_heads);
+  const int64_t mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
+  int* err = static_cast<int*>(workspace);
+  if (p.step) {
+    const AttnStepArgs a = {tq,
+                            attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads),
+                            attn_tensor(v, d.v_stride, d.batch, d.kv_tokens, d.kv_heads),
+                            to, kv_lens, key_mask, mask_sb, lse, err, d.q_tokens, d.kv_tokens,
+                            d.q_heads, d.kv_heads, d.head_dim, group, d.q_tokens * group, p.split,
+                            d.scale};
+    return d.dtype == DCNV2_BF16 ? launch_step<true>(a, p, dev, st)
+                                 : launch_step<false>(a, p, dev, st);
+  }
   AttnArgs a = {};
-  a.q = attn_tensor(q, d.q_stride, d.batch, d.q_tokens, d.q_heads);
-  a.o = attn_tensor(out, d.out_stride, d.batch, d.q_tokens, d.q_heads);
+  a.q = tq;
+  a.o = to;
   a.kv_lens = kv_lens;
   a.key_mask = key_mask;
-  a.mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
+  a.mask_sb = mask_sb;
   a.lse = lse;
-  a.err = static_cast<int*>(workspace);
+  a.err = err;
   a.L = d.q_tokens; a.S = d.kv_tokens; a.H = d.q_heads; a.G = d.kv_heads; a.D = d.head_dim;
-  a.group = d.q_heads / d.kv_heads;
-  a.rows = d.q_tokens * a.group;
+  a.group = group;
+  a.rows = d.q_tokens * group;
   a.row_tiles = p.row_tiles;
   a.split = p.split;
   a.scale = d.scale;
@@ -394,7 +448,6 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
              !attn_tensor_map(&mv, v, d.v_stride, d, &a.v_batch, &a.v_head)) {
     return DCNV2_ERR_UNSUPPORTED;  // strides of 2^40 bytes and more
   }
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return d.dtype == DCNV2_BF16 ? launch_attention<true>(a, mk, mv, p, dev, st)
                                : launch_attention<false>(a, mk, mv, p, dev, st);
 }
