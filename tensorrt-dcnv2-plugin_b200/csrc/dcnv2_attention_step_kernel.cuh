@@ -8,8 +8,9 @@
 // multiplies with m16n8k16 MMAs on 16 padded rows, and keeps its own maximum, sum and O in
 // registers, so that no barrier stands between the loads. Tensor-memory MMAs would need 128 rows
 // (or the states as rows) and barriers between the roles; at these sizes the tensor core is idle
-// most of the time either way. The warps' parts are joined in shared memory, those of the CTAs of a
-// cluster, which split the states, through distributed shared memory in a fixed order.
+// most of the time either way. The warps' parts are joined in shared memory; the CTAs of a cluster,
+// which split the states, send theirs to the CTA that finishes the element (stores into distributed
+// shared memory, one barrier), which adds them in a fixed order.
 //
 // States that are not kept are not read: their rows in shared memory are filled with zeros (the
 // copy's source size is 0), their scores are -inf; chunks without a kept state cost nothing.
@@ -25,6 +26,7 @@ namespace dcnv2 {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = kStepWarps * 32;
 constexpr int kStepRows = 16;
+constexpr int kStepMaxSplit = 16;  // CTAs of a cluster
 
 struct AttnStepArgs {
   AttnTensor q, k, v, o;
@@ -32,7 +34,6 @@ struct AttnStepArgs {
   const uint8_t* key_mask;
   int64_t mask_sb;
   float* lse;
-  int* err;
   int L, S, H, G, D;
   int group, rows;       // rows = L * group <= 16
   int split;             // CTAs of a cluster along the states
@@ -49,10 +50,13 @@ struct StepLayout {
   static constexpr uint32_t kStage = 2 * kTile;                   // K, V
   static constexpr uint32_t kWarp = kStages * kStage;             // 24 KB
   static constexpr uint32_t kBytes = kStepWarps * kWarp;
-  // at the end, over the rings: fp32 O of each warp [16][DP], then the CTA's; (max, sum) behind
+  // at the end, over the rings: fp32 O of each warp [16][DP]; behind them the warps' (max, sum),
+  // then what the CTAs of the cluster send: (max, sum) of all rows, O of the elements finished here
   static constexpr uint32_t kPart = kStepRows * DP * 4;
-  static constexpr uint32_t kStats = kBytes;                      // [kStepWarps + 1][16] float2
-  static constexpr uint32_t kTotal = kStats + (kStepWarps + 1) * kStepRows * 8;
+  static constexpr uint32_t kStats = kBytes;                      // [kStepWarps][16] float2
+  static constexpr uint32_t kSentStats = kStats + kStepWarps * kStepRows * 8;  // [split][16] float2
+  static constexpr uint32_t kSent = kSentStats + kStepMaxSplit * kStepRows * 8;
+  static constexpr uint32_t kTotal = kSent + kPart + kStepMaxSplit * 16;
   static_assert(kPart <= kWarp, "a warp's O fits over its ring");
 };
 
@@ -65,26 +69,42 @@ __device__ __forceinline__ uint32_t step_at(int r, int c) {
   return static_cast<uint32_t>(r) * (DP * 2) + (static_cast<uint32_t>(c ^ mix) << 4);
 }
 
-// Copies a chunk's rows j0 .. j0 + kKeys - 1 of both tensors; rows whose bit is not set, and elements
-// from D on, are filled with zeros.
+// The lane's part of copying a chunk: 16-byte piece c of rows r0, r0 + kRowsAtOnce, ...
 template <int DP>
-__device__ __forceinline__ void step_load(uint32_t dst, const uint16_t* k, const uint16_t* v,
-                                          int64_t kst, int64_t vst, int j0, uint64_t keep, int D,
-                                          int lane) {
-  using LY = StepLayout<DP>;
-  constexpr int kChunks = DP / 8, kRowsAtOnce = 32 / kChunks;
-  const int c = lane % kChunks;
-  const bool inside = c * 8 < D;
-#pragma unroll
-  for (int i = 0; i < LY::kKeys / kRowsAtOnce; ++i) {
-    const int r = i * kRowsAtOnce + lane / kChunks;
-    const bool take = inside && ((keep >> r) & 1);
-    const int64_t j = take ? j0 + r : 0;
-    const uint32_t at = dst + step_at<DP>(r, c);
-    ptx::cp_async_16(at, k + j * kst + (inside ? c * 8 : 0), take);
-    ptx::cp_async_16(at + LY::kTile, v + j * vst + (inside ? c * 8 : 0), take);
+struct StepCopy {
+  static constexpr int kChunks = DP / 8, kRowsAtOnce = 32 / kChunks;
+  static constexpr int kTimes = StepLayout<DP>::kKeys / kRowsAtOnce;
+  const uint16_t *k, *v;   // of row r0 of the first chunk
+  int64_t kst, vst;        // elements between the lane's rows
+  uint32_t r0;
+  uint32_t at;             // byte offset of row r0 in a tile, without the mixing
+  uint32_t c;
+  bool inside;             // the piece lies inside the head
+
+  __device__ __forceinline__ StepCopy(const uint16_t* kp, const uint16_t* vp, int64_t ks, int64_t vs,
+                                      int D, int lane)
+      : kst(ks * kRowsAtOnce), vst(vs * kRowsAtOnce), r0(lane / kChunks), c(lane % kChunks) {
+    inside = static_cast<int>(c) * 8 < D;
+    k = kp + r0 * ks + (inside ? c * 8 : 0);
+    v = vp + r0 * vs + (inside ? c * 8 : 0);
   }
-}
+  // The chunk whose first row is kKeys * chunk behind; rows whose bit is not set, and elements
+  // behind the head, are filled with zeros.
+  __device__ __forceinline__ void operator()(uint32_t dst, int chunk, uint64_t keep,
+                                             bool whole) const {
+    const uint16_t* kp = k + static_cast<int64_t>(chunk) * kTimes * kst;
+    const uint16_t* vp = v + static_cast<int64_t>(chunk) * kTimes * vst;
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+      const uint32_t to = dst + step_at<DP>(i * kRowsAtOnce + r0, c);
+      const bool take = inside && (whole || ((keep >> (i * kRowsAtOnce + r0)) & 1));
+      ptx::cp_async_16(to, take ? kp : k, take);  // (nothing is read where take is false)
+      ptx::cp_async_16(to + StepLayout<DP>::kTile, take ? vp : v, take);
+      kp += kst;
+      vp += vst;
+    }
+  }
+};
 
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(kStepThreads)
@@ -101,8 +121,8 @@ __global__ void __launch_bounds__(kStepThreads)
   const int unit = static_cast<int>(blockIdx.x) / args.split;
   const int g = unit % args.G, b = unit / args.G;
   ptx::griddep_launch_dependents();
+  if (args.split > 1) ptx::cluster_arrive();  // waited for before anything is sent to a CTA
   ptx::griddep_wait();
-  if (threadIdx.x == 0) args.err[blockIdx.x] = 0;  // nothing here waits without end
 
   int len = args.S;
   if (args.kv_lens) len = max(0, min(len, __ldg(args.kv_lens + b)));
@@ -117,38 +137,30 @@ __global__ void __launch_bounds__(kStepThreads)
   const uint32_t ring = base + warp * LY::kWarp;
 
   // bits of the kept states of a chunk; the lane's mask bytes are fetched a chunk ahead
+  constexpr uint64_t kWhole = KEYS == 64 ? ~0ull : (1ull << (KEYS & 63)) - 1;
   uint8_t ahead[2] = {0, 0};
   auto fetch_mask = [&](int chunk) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int r = x * 32 + lane, j = chunk * KEYS + r;
-      ahead[x] = mask && chunk < c1 && r < KEYS && j < len ? __ldg(mask + j) : 0;
+      ahead[x] = chunk < c1 && r < KEYS && j < len ? __ldg(mask + j) : 0;
     }
   };
-  auto keep_bits = [&](int chunk) -> uint64_t {
-    const int left = len - chunk * KEYS;
-    uint64_t bits = left >= KEYS ? (KEYS == 64 ? ~0ull : (1ull << KEYS) - 1) : (1ull << left) - 1;
-    if (mask) {
-      const uint64_t lo = __ballot_sync(0xffffffffu, ahead[0] != 0);
-      const uint64_t hi = KEYS > 32 ? __ballot_sync(0xffffffffu, ahead[1] != 0) : 0;
-      bits &= lo | hi << 32;
-    }
-    return bits;
-  };
+  const StepCopy<DP> copy(k, v, args.k.st, args.v.st, args.D, lane);
   uint64_t kept[NS];  // of the chunks in the ring
   int next = c0;      // chunk that is loaded next
   auto load = [&](int stage) -> uint64_t {
     uint64_t bits = 0;
     if (next < c1) {
+      const int left = len - next * KEYS;
+      bits = left >= KEYS ? kWhole : (1ull << left) - 1;
       if (mask) {
-        bits = keep_bits(next);
+        const uint64_t lo = __ballot_sync(0xffffffffu, ahead[0] != 0);
+        const uint64_t hi = KEYS > 32 ? __ballot_sync(0xffffffffu, ahead[1] != 0) : 0;
+        bits &= lo | hi << 32;
         fetch_mask(next + 1);
-      } else {
-        bits = keep_bits(next);
       }
-      if (bits)
-        step_load<DP>(ring + stage * LY::kStage, k, v, args.k.st, args.v.st, next * KEYS, bits,
-                      args.D, lane);
+      if (bits) copy(ring + stage * LY::kStage, next, bits, bits == kWhole);
       ++next;
     }
     ptx::cp_async_commit();
@@ -195,38 +207,51 @@ __global__ void __launch_bounds__(kStepThreads)
     stage = stage + 1 == NS ? 0 : stage + 1;
     if (!bits) continue;
 
-    float s[NT][4];
+    // two accumulators per score tile (even and odd k-steps), so that MMAs do not wait for one
+    // another
+    constexpr int CH = KT >= 4 ? 2 : 1;
+    float s2[CH][NT][4];
 #pragma unroll
-    for (int x = 0; x < NT; ++x)
+    for (int z = 0; z < CH; ++z)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) s[x][y] = 0.f;
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s2[z][x][y] = 0.f;
 #pragma unroll
     for (int x = 0; x < KT; ++x)
 #pragma unroll
       for (int y = 0; y < NT; y += 2) {
-        // four 8x8 tiles: states 8 y .. 8 y + 15 (lanes 0-15: chunk 2 x, 16-31: chunk 2 x + 1)
+        // four 8x8 tiles: states 8 y .. 8 y + 15 (lanes 0-15: piece 2 x, 16-31: piece 2 x + 1)
         uint32_t f[4];
         ptx::ldmatrix_x4(f, kt + step_at<DP>(y * 8 + (lane & 15), 2 * x + (lane >> 4)));
-        ptx::mma_16816<BF16>(s[y], qf[x], f[0], f[2]);
-        ptx::mma_16816<BF16>(s[y + 1], qf[x], f[1], f[3]);
+        ptx::mma_16816<BF16>(s2[x % CH][y], qf[x], f[0], f[2]);
+        ptx::mma_16816<BF16>(s2[x % CH][y + 1], qf[x], f[1], f[3]);
       }
-    if (bits != (KEYS == 64 ? ~0ull : (1ull << KEYS) - 1)) {
+    float (&s)[NT][4] = s2[0];
 #pragma unroll
-      for (int x = 0; x < NT; ++x)
+    for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if (!((bits >> (x * 8 + t4 * 2 + (y & 1))) & 1)) s[x][y] = -INFINITY;
-    }
-    // per row half (rows g4, g4 + 8): the chunk's maximum over the quad
+      for (int y = 0; y < 4; ++y) {
+        if constexpr (CH == 2) s[x][y] += s2[1][x][y];
+        if (bits != kWhole && !((bits >> (x * 8 + t4 * 2 + (y & 1))) & 1)) s[x][y] = -INFINITY;
+      }
+    // the lane's maximum of rows g4 and g4 + 8; the quad's is needed only where a row's reference
+    // has to move
+    float top[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float top = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+      top[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
 #pragma unroll
-      for (int x = 1; x < NT; ++x) top = fmaxf(top, fmaxf(s[x][2 * r], s[x][2 * r + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float m = fmaxf(m_ref[r], top);
-      if (__any_sync(0xffffffffu, (m - m_ref[r]) * c > kAttnLazy)) {
+      for (int x = 1; x < NT; ++x) top[r] = fmaxf(top[r], fmaxf(s[x][2 * r], s[x][2 * r + 1]));
+    }
+    // ((-inf) - (-inf) is NaN, which is not greater)
+    if (__any_sync(0xffffffffu, (top[0] - m_ref[0]) * c > kAttnLazy ||
+                                    (top[1] - m_ref[1]) * c > kAttnLazy)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m = fmaxf(m_ref[r], top[r]);
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
         const float fac = m == m_ref[r] ? 1.f : ptx::ex2((m_ref[r] - m) * c);
         l[r] *= fac;
         m_ref[r] = m;
@@ -236,13 +261,18 @@ __global__ void __launch_bounds__(kStepThreads)
           o[x][2 * r + 1] *= fac;
         }
       }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
       const float neg = (m_ref[r] == -INFINITY ? 0.f : -m_ref[r] * c) + shift;
+      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         s[x][2 * r] = ptx::ex2(fmaf(s[x][2 * r], c, neg));
         s[x][2 * r + 1] = ptx::ex2(fmaf(s[x][2 * r + 1], c, neg));
-        l[r] += s[x][2 * r] + s[x][2 * r + 1];
+        sum[x & 1] += s[x][2 * r] + s[x][2 * r + 1];
       }
+      l[r] += sum[0] + sum[1];
     }
 #pragma unroll
     for (int x = 0; x < KEYS / 16; ++x) {
@@ -290,7 +320,10 @@ __global__ void __launch_bounds__(kStepThreads)
       args.lse[(static_cast<int64_t>(b) * args.H + h) * args.L + tok] =
           total == 0.f ? -INFINITY : kLn2 * (top * c - shift + log2f(total));
   };
+  // element quad x is finished by CTA x % split, as its element quad x / split
   const int quads = args.D / 4, items = args.rows * quads;
+  const int mine = (items + args.split - 1) / args.split;
+  if (args.split > 1) ptx::cluster_wait();
   for (int x = threadIdx.x; x < items; x += kStepThreads) {
     const int r = x / quads, d = (x - r * quads) * 4;
     float top = -INFINITY, total = 0.f;
@@ -310,26 +343,28 @@ __global__ void __launch_bounds__(kStepThreads)
     if (args.split == 1) {
       store(r, d, acc, top, total);
     } else {
-      // over the first warp's part: each place is read and written by this thread alone
-      *reinterpret_cast<float4*>(step_smem + (r * DP + d) * 4) = acc;
-      if (d == 0) stats[kStepWarps * kStepRows + r] = make_float2(top, total);
+      const int to = x % args.split, at = x / args.split;
+      ptx::st_cluster_f4(ptx::mapa_shared(base + LY::kSent + (rank * mine + at) * 16, to), acc);
+      if (d == 0)
+        for (int y = 0; y < args.split; ++y)
+          ptx::st_cluster_f2(
+              ptx::mapa_shared(base + LY::kSentStats + (rank * kStepRows + r) * 8, y),
+              make_float2(top, total));
     }
   }
   if (args.split > 1) {
     // ---------------------------------------------------------- parts of the CTAs
-    ptx::cluster_sync();
-    for (int x = rank * kStepThreads + static_cast<int>(threadIdx.x); x < items;
-         x += args.split * kStepThreads) {
-      const int r = x / quads, d = (x - r * quads) * 4;
-      const uint32_t st = base + LY::kStats + (kStepWarps * kStepRows + r) * 8;
+    ptx::cluster_sync();  // all has arrived; nothing is sent from here on
+    const float2* ml_of = reinterpret_cast<const float2*>(step_smem + LY::kSentStats);
+    const float4* sent = reinterpret_cast<const float4*>(step_smem + LY::kSent);
+    for (int at = threadIdx.x; at < mine && at * args.split + rank < items; at += kStepThreads) {
+      const int x = at * args.split + rank, r = x / quads, d = (x - r * quads) * 4;
       float top = -INFINITY, total = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int y = 0; y < args.split; ++y)
-        top = fmaxf(top, ptx::ld_cluster_f2(ptx::mapa_shared(st, y)).x);
-#pragma unroll 4
+      for (int y = 0; y < args.split; ++y) top = fmaxf(top, ml_of[y * kStepRows + r].x);
       for (int y = 0; y < args.split; ++y) {
-        const float2 ml = ptx::ld_cluster_f2(ptx::mapa_shared(st, y));
-        const float4 q = ptx::ld_cluster_f4(ptx::mapa_shared(base + (r * DP + d) * 4, y));
+        const float2 ml = ml_of[y * kStepRows + r];
+        const float4 q = sent[y * mine + at];
         const float f = ml.x == top ? 1.f : ptx::ex2((ml.x - top) * c);
         total = fmaf(ml.y, f, total);
         acc.x = fmaf(q.x, f, acc.x); acc.y = fmaf(q.y, f, acc.y);
@@ -337,7 +372,6 @@ __global__ void __launch_bounds__(kStepThreads)
       }
       store(r, d, acc, top, total);
     }
-    ptx::cluster_sync();  // the parts stay until every CTA has read them
   }
 }
 

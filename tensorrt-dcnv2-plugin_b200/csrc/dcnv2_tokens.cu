@@ -197,14 +197,8 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   if (rows > INT_MAX - 2 * kAttnTile) return DCNV2_ERR_INVALID_ARG;
   p->step = rows <= kStepRows;
   if (p->step) {
-    const int64_t units = int64_t(d->batch) * d->kv_heads;
-    const int keys = d->head_dim > 64 ? 16 : d->head_dim > 32 ? 32 : 64;
-    p->split = 1;
-    while (p->split < kAttnMaxSplit && units * p->split < 4 * kPlanSms &&
-           cdiv(d->kv_tokens, keys) >= int64_t(p->split) * 2 * kStepWarps * 2)
-      p->split *= 2;
-    if (units * p->split > INT_MAX) return DCNV2_ERR_INVALID_ARG;
-    p->grid = static_cast<unsigned>(units * p->split);
+    if (int64_t(d->batch) * d->kv_heads * kStepMaxSplit > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+    p->grid = 0;  // no error words: nothing in the kernel waits for another role
     return DCNV2_OK;
   }
   p->paired = rows <= kAttnTile;
@@ -282,28 +276,48 @@ dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CU
                   : launch_attention<64, false, BF16>(a, mk, mv, p, dev, st);
 }
 
+// CTAs of a cluster that split the states of one (sequence, kv head): as few as give every SM a CTA,
+// with a chunk for each of their warps. One CTA draws at most about 50 GB/s, so that fewer CTAs than
+// SMs leave bandwidth unused, while more cost their start and end again (32 x 8 heads of 32, 5456
+// states: 256 CTAs 32 us, 512 36 us, 1024 45 us; 8 kv heads of 128, 5456 states: 64 CTAs 12.9 us, 128
+// 10.7 us). Lengths of their own leave SMs idle behind the short sequences; twice the CTAs even that
+// out (8 x 8 heads of 128, up to 60001 states: 128 CTAs 245 us, 512 210 us).
+int step_split(int64_t units, const AttnStepArgs& a, int sm_count) {
+  const int keys = a.D > 64 ? 16 : a.D > 32 ? 32 : 64;
+  const int64_t want = int64_t(sm_count) * (a.kv_lens ? 2 : 1);
+  int split = 1;
+  while (split < kStepMaxSplit && units * split < want &&
+         cdiv(a.S, keys) >= int64_t(split) * 2 * kStepWarps)
+    split *= 2;
+  return split;
+}
+
 template <int DP, bool BF16>
-dcnv2_status launch_step(const AttnStepArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
+dcnv2_status launch_step(const AttnStepArgs& a, int64_t units, int dev, cudaStream_t st) {
   auto kernel = dcnv2_attention_step_kernel<DP, BF16>;
   constexpr size_t smem = StepLayout<DP>::kTotal;
+  static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs per SM");
   static std::atomic<bool> set[kMaxDevices];  // per device; setting it twice does no harm
   if (!set[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(smem));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(smem));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return launched(e);
     set[dev].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      launch_config(p.grid, kStepThreads, smem, st, at, static_cast<unsigned>(p.split));
+      launch_config(static_cast<unsigned>(units * a.split), kStepThreads, smem, st, at,
+                    static_cast<unsigned>(a.split));
   return launched(cudaLaunchKernelEx(&cfg, kernel, a));
 }
 
 template <bool BF16>
-dcnv2_status launch_step(const AttnStepArgs& a, const AttnPlan& p, int dev, cudaStream_t st) {
-  return a.D > 64   ? launch_step<128, BF16>(a, p, dev, st)
-         : a.D > 32 ? launch_step<64, BF16>(a, p, dev, st)
-                    : launch_step<32, BF16>(a, p, dev, st);
+dcnv2_status launch_step(const AttnStepArgs& a, int64_t units, int dev, cudaStream_t st) {
+  return a.D > 64   ? launch_step<128, BF16>(a, units, dev, st)
+         : a.D > 32 ? launch_step<64, BF16>(a, units, dev, st)
+                    : launch_step<32, BF16>(a, units, dev, st);
 }
 
 }  // namespace
@@ -416,14 +430,15 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
   const int64_t mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
   int* err = static_cast<int*>(workspace);
   if (p.step) {
-    const AttnStepArgs a = {tq,
-                            attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads),
-                            attn_tensor(v, d.v_stride, d.batch, d.kv_tokens, d.kv_heads),
-                            to, kv_lens, key_mask, mask_sb, lse, err, d.q_tokens, d.kv_tokens,
-                            d.q_heads, d.kv_heads, d.head_dim, group, d.q_tokens * group, p.split,
-                            d.scale};
-    return d.dtype == DCNV2_BF16 ? launch_step<true>(a, p, dev, st)
-                                 : launch_step<false>(a, p, dev, st);
+    AttnStepArgs a = {tq,
+                      attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads),
+                      attn_tensor(v, d.v_stride, d.batch, d.kv_tokens, d.kv_heads),
+                      to, kv_lens, key_mask, mask_sb, lse, d.q_tokens, d.kv_tokens, d.q_heads,
+                      d.kv_heads, d.head_dim, group, d.q_tokens * group, 1, d.scale};
+    const int64_t units = int64_t(d.batch) * d.kv_heads;
+    a.split = step_split(units, a, di->sm_count);
+    return d.dtype == DCNV2_BF16 ? launch_step<true>(a, units, dev, st)
+                                 : launch_step<false>(a, units, dev, st);
   }
   AttnArgs a = {};
   a.q = tq;
@@ -462,7 +477,7 @@ dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int32_t bits = 0;
   const int* words = static_cast<const int*>(workspace);
-  for (unsigned at = 0; at < p.grid;) {
+  for (unsigned at = 0; at < p.grid;) {  // (none for a few rows)
     int32_t part[1024];
     const unsigned n = p.grid - at < 1024u ? p.grid - at : 1024u;
     if (cudaMemcpyAsync(part, words + at, n * sizeof(int), cudaMemcpyDeviceToHost, st) !=
