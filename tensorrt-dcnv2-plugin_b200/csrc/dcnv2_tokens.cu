@@ -164,12 +164,12 @@ struct AttnPlan {
   bool step = false;       // few rows: dcnv2_attention_step_kernel
   bool paired = false;     // one tile of rows, the warpgroups alternate over the states
   bool wide = false;       // heads of more than 64 elements
-  int row_tiles = 0, split = 1;
+  int heads = 1, kv_parts = 1, tile_tokens = 1;  // rows of a tile (AttnArgs)
+  int row_tiles = 0, items = 0, split = 1;
   unsigned grid = 0;
 };
 
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
-constexpr int kAttnMaxSplit = 8;  // portable cluster size
 
 dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   if (!d) return DCNV2_ERR_INVALID_ARG;
@@ -186,6 +186,8 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
         !stride_ok(d->k_stride[j], kx[j]) || !stride_ok(d->v_stride[j], kx[j]))
       return DCNV2_ERR_INVALID_ARG;
     if (qx[j] > 1 && (d->q_stride[j] % 8 || d->out_stride[j] % 8)) return DCNV2_ERR_UNSUPPORTED;
+    if (j > 0 && qx[j] > 1 && !d->q_stride[j]) return DCNV2_ERR_UNSUPPORTED;
+    if (j == 1 && kx[j] > 1 && (!d->k_stride[j] || !d->v_stride[j])) return DCNV2_ERR_UNSUPPORTED;
     if (kx[j] > 1 && (d->k_stride[j] % 8 || d->v_stride[j] % 8)) return DCNV2_ERR_UNSUPPORTED;
     // outputs of two rows at one place would race
     if (qx[j] > 1 && d->out_stride[j] < d->head_dim && d->batch && d->q_tokens)
@@ -193,7 +195,8 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   }
   if (!stride_ok(d->mask_batch_stride, d->batch)) return DCNV2_ERR_INVALID_ARG;
   p->wide = d->head_dim > 64;
-  const int64_t rows = int64_t(d->q_tokens) * (d->q_heads / d->kv_heads);
+  const int group = d->q_heads / d->kv_heads;
+  const int64_t rows = int64_t(d->q_tokens) * group;
   if (rows > INT_MAX - 2 * kAttnTile) return DCNV2_ERR_INVALID_ARG;
   p->step = rows <= kStepRows;
   if (p->step) {
@@ -201,16 +204,24 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
     p->grid = 0;  // no error words: nothing in the kernel waits for another role
     return DCNV2_OK;
   }
-  p->paired = rows <= kAttnTile;
-  p->row_tiles = static_cast<int>(cdiv(rows, p->paired ? kAttnTile : 2 * kAttnTile));
-  const int64_t ctas = int64_t(d->batch) * d->kv_heads * p->row_tiles;
+  for (p->heads = group < kAttnTile ? group : kAttnTile; group % p->heads;) --p->heads;
+  p->kv_parts = group / p->heads;
+  p->tile_tokens = kAttnTile / p->heads;
+  p->paired = d->q_tokens <= p->tile_tokens;
+  p->row_tiles = static_cast<int>(cdiv(d->q_tokens, p->tile_tokens * (p->paired ? 1 : 2)));
+  const int64_t groups = int64_t(d->kv_heads) * p->kv_parts;
+  if (groups > INT_MAX || int64_t(d->batch) * groups > INT_MAX) return DCNV2_ERR_INVALID_ARG;
+  const int64_t ctas = int64_t(d->batch) * groups * p->row_tiles;
   // Split the states over as many CTAs as still run at once, each with a tile at least.
   p->split = 1;
   while (p->split < kAttnMaxSplit && ctas * p->split * 2 <= kPlanSms &&
          cdiv(d->kv_tokens, kAttnTile) >= int64_t(p->split) * 2 * (p->paired ? 2 : 1))
     p->split *= 2;
   if (ctas * p->split > INT_MAX) return DCNV2_ERR_INVALID_ARG;
-  p->grid = static_cast<unsigned>(ctas * p->split);
+  p->items = static_cast<int>(ctas);
+  // items that are not split or joined are taken in turn by one CTA per SM
+  const int64_t most = p->paired || p->split > 1 ? ctas : kPlanSms;
+  p->grid = static_cast<unsigned>((ctas < most ? ctas : most) * p->split);
   return DCNV2_OK;
 }
 
@@ -221,11 +232,23 @@ AttnTensor attn_tensor(const void* p, const int64_t (&stride)[3], int64_t batch,
                     heads > 1 ? stride[2] : 0};
 }
 
+bool encode_map(CUtensorMap* m, const void* p, int rank, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box) {
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  std::memset(m, 0, sizeof(*m));
+  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  return encode &&
+         encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(p), dims, strides, box,
+                ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x 128 tokens in the
 // 128-byte swizzle. Axes that no step is taken along, or that share their states, have extent 1.
 // What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
-bool attn_tensor_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
-                     const dcnv2_attention_desc& d, int* batch_step, int* head_step) {
+bool states_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
+                const dcnv2_attention_desc& d, int* batch_step, int* head_step) {
   const bool heads = d.kv_heads > 1 && stride[2] > 0, batch = d.batch > 1 && stride[0] > 0;
   *head_step = heads;
   *batch_step = batch;
@@ -237,19 +260,40 @@ bool attn_tensor_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
   const cuuint64_t strides[3] = {d.kv_tokens > 1 ? static_cast<cuuint64_t>(stride[1]) * 2 : row,
                                  heads ? static_cast<cuuint64_t>(stride[2]) * 2 : row,
                                  batch ? static_cast<cuuint64_t>(stride[0]) * 2 : row};
-  const cuuint32_t box[4] = {64, kAttnTile, 1, 1}, ones[4] = {1, 1, 1, 1};
-  std::memset(m, 0, sizeof(*m));
-  PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
-  return encode &&
-         encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(p), dims, strides, box, ones,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[4] = {64, kAttnTile, 1, 1};
+  return encode_map(m, p, 4, dims, strides, box);
 }
 
+// Tensor map of q or out: (element, head of the group, token, group, batch), boxes of 64 elements x
+// the rows of a tile.
+bool rows_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
+              const dcnv2_attention_desc& d, const AttnPlan& plan, int* batch_step) {
+  const int64_t groups = int64_t(d.q_heads) / plan.heads;
+  const bool batch = d.batch > 1 && stride[0] > 0;
+  *batch_step = batch;
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(d.head_dim),
+                              static_cast<cuuint64_t>(plan.heads),
+                              static_cast<cuuint64_t>(d.q_tokens),
+                              static_cast<cuuint64_t>(groups),
+                              static_cast<cuuint64_t>(batch ? d.batch : 1)};
+  const cuuint64_t row = static_cast<cuuint64_t>(d.head_dim) * 2;
+  const cuuint64_t head = d.q_heads > 1 ? static_cast<cuuint64_t>(stride[2]) * 2 : row;
+  const cuuint64_t strides[4] = {head,
+                                 d.q_tokens > 1 ? static_cast<cuuint64_t>(stride[1]) * 2 : row,
+                                 head * plan.heads,
+                                 batch ? static_cast<cuuint64_t>(stride[0]) * 2 : row};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(plan.heads),
+                             static_cast<cuuint32_t>(plan.tile_tokens), 1, 1};
+  return encode_map(m, p, 5, dims, strides, box);
+}
+
+struct AttnMaps {
+  CUtensorMap q, k, v, o;
+};
+
 template <int DP, bool PAIRED, bool BF16>
-dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
-                              const AttnPlan& p, int dev, cudaStream_t st) {
+dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPlan& p, int dev,
+                              cudaStream_t st) {
   auto kernel = dcnv2_cross_attention_kernel<DP, PAIRED, BF16>;
   constexpr size_t smem = attn_smem_bytes<DP, PAIRED>();
   static_assert(smem <= kSmemLimit, "shared memory");
@@ -263,17 +307,17 @@ dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CU
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
       launch_config(p.grid, kAttnThreads, smem, st, at, static_cast<unsigned>(p.split));
-  return launched(cudaLaunchKernelEx(&cfg, kernel, a, mk, mv));
+  return launched(cudaLaunchKernelEx(&cfg, kernel, a, m.q, m.k, m.v, m.o));
 }
 
 template <bool BF16>
-dcnv2_status launch_attention(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
-                              const AttnPlan& p, int dev, cudaStream_t st) {
+dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPlan& p, int dev,
+                              cudaStream_t st) {
   if (p.wide)
-    return p.paired ? launch_attention<128, true, BF16>(a, mk, mv, p, dev, st)
-                    : launch_attention<128, false, BF16>(a, mk, mv, p, dev, st);
-  return p.paired ? launch_attention<64, true, BF16>(a, mk, mv, p, dev, st)
-                  : launch_attention<64, false, BF16>(a, mk, mv, p, dev, st);
+    return p.paired ? launch_attention<128, true, BF16>(a, m, p, dev, st)
+                    : launch_attention<128, false, BF16>(a, m, p, dev, st);
+  return p.paired ? launch_attention<64, true, BF16>(a, m, p, dev, st)
+                  : launch_attention<64, false, BF16>(a, m, p, dev, st);
 }
 
 // CTAs of a cluster that split the states of one (sequence, kv head): as few as give every SM a CTA,
@@ -428,7 +472,6 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
   const AttnTensor tq = attn_tensor(q, d.q_stride, d.batch, d.q_tokens, d.q_heads);
   const AttnTensor to = attn_tensor(out, d.out_stride, d.batch, d.q_tokens, d.q_heads);
   const int64_t mask_sb = d.batch > 1 ? d.mask_batch_stride : 0;
-  int* err = static_cast<int*>(workspace);
   if (p.step) {
     AttnStepArgs a = {tq,
                       attn_tensor(k, d.k_stride, d.batch, d.kv_tokens, d.kv_heads),
@@ -441,30 +484,36 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
                                  : launch_step<false>(a, units, dev, st);
   }
   AttnArgs a = {};
-  a.q = tq;
-  a.o = to;
   a.kv_lens = kv_lens;
   a.key_mask = key_mask;
   a.mask_sb = mask_sb;
   a.lse = lse;
-  a.err = err;
-  a.L = d.q_tokens; a.S = d.kv_tokens; a.H = d.q_heads; a.G = d.kv_heads; a.D = d.head_dim;
-  a.group = group;
-  a.rows = d.q_tokens * group;
+  a.out = out;
+  a.out_sb = to.sb; a.out_st = to.st; a.out_sh = to.sh;
+  a.err = static_cast<int*>(workspace);
+  a.L = d.q_tokens; a.S = d.kv_tokens; a.H = d.q_heads; a.D = d.head_dim;
+  a.heads = p.heads;
+  a.kv_parts = p.kv_parts;
+  a.groups = d.kv_heads * p.kv_parts;
+  a.tile_tokens = p.tile_tokens;
   a.row_tiles = p.row_tiles;
+  a.items = p.items;
   a.split = p.split;
   a.scale = d.scale;
   a.timeout_ns = kDefaultTimeoutNs;
-  CUtensorMap mk, mv;
-  if (d.kv_tokens == 0) {  // nothing is loaded
-    std::memset(&mk, 0, sizeof(mk));
-    mv = mk;
-  } else if (!attn_tensor_map(&mk, k, d.k_stride, d, &a.k_batch, &a.k_head) ||
-             !attn_tensor_map(&mv, v, d.v_stride, d, &a.v_batch, &a.v_head)) {
+  AttnMaps m;
+  int out_batch = 0;
+  if (!rows_map(&m.q, q, d.q_stride, d, p, &a.q_batch) ||
+      !rows_map(&m.o, out, d.out_stride, d, p, &out_batch))
     return DCNV2_ERR_UNSUPPORTED;  // strides of 2^40 bytes and more
+  if (d.kv_tokens == 0) {  // nothing is loaded
+    m.k = m.v = m.q;
+  } else if (!states_map(&m.k, k, d.k_stride, d, &a.k_batch, &a.k_head) ||
+             !states_map(&m.v, v, d.v_stride, d, &a.v_batch, &a.v_head)) {
+    return DCNV2_ERR_UNSUPPORTED;
   }
-  return d.dtype == DCNV2_BF16 ? launch_attention<true>(a, mk, mv, p, dev, st)
-                               : launch_attention<false>(a, mk, mv, p, dev, st);
+  return d.dtype == DCNV2_BF16 ? launch_attention<true>(a, m, p, dev, st)
+                               : launch_attention<false>(a, m, p, dev, st);
 }
 
 dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
