@@ -269,7 +269,8 @@ typedef struct {
   int64_t mask_batch_stride;     /* bytes between the sequences of key_mask; 0: shared */
 } dcnv2_attention_desc;
 
-/* Workspace bytes of dcnv2_cross_attention (its error words). Returns 0 on a bad desc. */
+/* Workspace bytes of dcnv2_cross_attention (its error words): 0 when it needs none (up to 16 query
+ * rows per kv head: no wait can run out there; workspace may be NULL), and on a bad desc. */
 DCNV2_API size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc* desc);
 
 /* out = softmax(scale * q k^T over the kept keys) v, each query row over all kept states of its

@@ -26,9 +26,9 @@
 // workspace, and the order of the sums is fixed.
 //
 // Roles (384 threads): warps 0-3 and 4-7 softmax and epilogue, warp 8 producer (kept-state words of
-// each tile, TMA of K and V; tiles without a kept state are left out altogether), warps 9 and 10
-// issue the MMAs of one softmax warpgroup each (and its Q), warp 11 zeroes the V rows of states that
-// are not kept (their probability is 0, but 0 * NaN is not). Warps whose rows lie behind the last
+// each tile, TMA of K and V; tiles without a kept state are left out altogether), warp 9
+// issues the MMAs (and loads Q), warp 10 zeroes the V rows of states that are not kept (their
+// probability is 0, but 0 * NaN is not). Warps whose rows lie behind the last
 // query skip their exponentials. Every wait is bounded.
 #pragma once
 #include <cuda.h>
@@ -38,6 +38,9 @@
 #include <stdint.h>
 
 #include "../../include/dcnv2.h"
+#ifndef FMAP
+#define FMAP 0
+#endif
 #include "dcnv2_wait.cuh"
 #include "ptx_sm100.cuh"
 
@@ -45,10 +48,11 @@ namespace dcnv2 {
 
 constexpr int kAttnTile = 128;                 // states per tile, rows per MMA
 constexpr int kAttnThreads = 12 * 32;
-constexpr int kAttnProducerWarp = 8, kAttnMmaWarp = 9, kAttnFixWarp = 11;  // MMA: 9 and 10
+constexpr int kAttnProducerWarp = 8, kAttnMmaWarp = 9, kAttnFixWarp = 10;  // (11 only fills up)
 constexpr uint32_t kAttnBlockBytes = kAttnTile * 128;  // 128 rows of one 128-byte swizzle block
 constexpr int kAttnMaxSplit = 8;               // CTAs of a cluster (portable size)
 constexpr float kAttnLazy = 8.f;               // log2 of the growth that rescales
+constexpr uint32_t kAttnFmaPairs = FMAP;     // of 16 pairs of exponentials, those on the FMA units
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnTensor {
@@ -96,8 +100,8 @@ struct AttnLayout {
   static constexpr uint32_t kInfo =                               // kInfos x 32 bytes
       kV + kStages * kTileBytes + (kOutBeside ? 2 * kTileBytes : 0);
   static constexpr uint32_t kBars = kInfo + kInfos * 32;
-  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 14;
-  static constexpr uint32_t kDrain = kBars + (kNumBars - 2) * 8;  // [2] the MMA issuers' own
+  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 11;
+  static constexpr uint32_t kDrain = kBars + (kNumBars - 1) * 8;  // the MMA issuer's own
   static constexpr uint32_t kFlags = kBars + kNumBars * 8;        // [kStages] of the K tiles
   static constexpr uint32_t kSlot = kFlags + kStages * 4;         // TMEM address, abort flag
   static constexpr uint32_t kBytes = kSlot + 16;
@@ -117,6 +121,27 @@ constexpr size_t attn_smem_bytes() {
 template <int DP>
 __device__ __forceinline__ uint32_t attn_part_at(int r, int c) {
   return static_cast<uint32_t>(r) * (DP * 4) + (static_cast<uint32_t>(c ^ (r & 7)) << 4);
+}
+
+// 2^x of two values on the FMA units, for the share of the exponentials that the special-function
+// units (16 per clock and SM) have no time for: x = n + f with n the nearest integer (taken from the
+// low bits of x + 1.5 * 2^23), 2^f by the polynomial of degree 5 whose relative error on [-1/2, 1/2] is
+// least (7.5e-8, found by Remez exchange), n added to the exponent. x is at most 15 here; below -126
+// the result is 2^-126 and less than 10^-37 of the row's largest.
+__device__ __forceinline__ float2 attn_exp2(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = ptx::add2(x, make_float2(12582912.f, 12582912.f));
+  const float2 f =
+      ptx::fma2(ptx::add2(t, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), x);
+  float2 p = ptx::fma2(f, make_float2(0.0013276472454890609f, 0.0013276472454890609f),
+                       make_float2(0.009675540961325169f, 0.009675540961325169f));
+  p = ptx::fma2(p, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
+  p = ptx::fma2(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+  p = ptx::fma2(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+  p = ptx::fma2(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // What the producer says of a tile, beside its kept-state words.
@@ -148,8 +173,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t info_full = v_empty + 8 * NS;         // [NI] words and flags of a tile
   const uint32_t info_empty = info_full + 8 * NI;      // [NI] read by everyone
   const uint32_t s_full = info_empty + 8 * NI;         // [2] scores of warpgroup w
-  const uint32_t p_half = s_full + 16;                 // [2] its first 64 probabilities
-  const uint32_t p_ready = p_half + 16;                // [2] all of them
+  const uint32_t p_ready = s_full + 16;                // [2] its probabilities
   const uint32_t q_full = p_ready + 16;                // [2] Q tile of warpgroup w
   const uint32_t q_empty = q_full + 16;                // [2] its last scores done
   const uint32_t o_full = q_empty + 16;                // [2] O of warpgroup w complete
@@ -184,10 +208,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       ptx::mbar_init(k_full + 8 * i, 1);
-      ptx::mbar_init(k_empty + 8 * i, PAIRED ? 1 : 2);
+      ptx::mbar_init(k_empty + 8 * i, 1);
       ptx::mbar_init(v_full + 8 * i, 1);
       ptx::mbar_init(v_ready + 8 * i, 1);
-      ptx::mbar_init(v_empty + 8 * i, PAIRED ? 1 : 2);
+      ptx::mbar_init(v_empty + 8 * i, 1);
     }
     for (int i = 0; i < NI; ++i) {
       ptx::mbar_init(info_full + 8 * i, 1);
@@ -195,14 +219,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(s_full + 8 * i, 1);
-      ptx::mbar_init(p_half + 8 * i, 4);
       ptx::mbar_init(p_ready + 8 * i, 4);
       ptx::mbar_init(q_full + 8 * i, 1);
       ptx::mbar_init(q_empty + 8 * i, 1);
       ptx::mbar_init(o_full + 8 * i, 1);
     }
     ptx::mbar_init(base + LY::kDrain, 1);
-    ptx::mbar_init(base + LY::kDrain + 8, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -219,7 +241,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t tmem = *slot;
   // tensor memory: scores of warpgroup w at 128 w (the probabilities over their first half), its O
   // at 256 + DP w
-  const int w = warp < 8 ? warp >> 2 : warp - kAttnMmaWarp;  // softmax warpgroup (or its issuer)
+  const int w = warp >> 2;  // softmax warpgroup
   const float c = args.scale * kLog2e;
   // fp16 probabilities are scaled by 2^7 (at most 2^15): small ones keep their bits longer
   const float shift = BF16 ? 0.f : 7.f;
@@ -334,7 +356,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     if (lane == 0) {
       int end = i;
-      for (; ok && end < i + (PAIRED ? 2 : 1); ++end) {  // the end, for each issuer
+      for (; ok && end < i + 1; ++end) {  // the end
         ok = wait_bar<kSuspend>(k_empty + 8 * (end % NS),
                                 (static_cast<uint32_t>(end / NS) & 1u) ^ 1u, wc,
                                 DCNV2_DEVERR_TIMEOUT_PRODUCER);
@@ -350,30 +372,28 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         drain_bar(v_full + 8 * (x % NS), static_cast<uint32_t>(x / NS) & 1u, wc);
       if (k_ahead) drain_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc);
     }
-  } else if (warp < kAttnFixWarp) {
-    // ------------------------------------------------------------ MMA issuer of warpgroup w
+  } else if (warp == kAttnMmaWarp) {
+    // ------------------------------------------------------------ MMA issuer
     // The warp runs this code as a whole, one elected lane issues. As little as possible stands between
     // the arrival of probabilities and the MMAs they release: what the next tile is, and that its K is
-    // there, is found out while the softmax works.
+    // there, is found out while the softmax works. One issuer serves the warpgroups in turn, which
+    // keeps them apart: two of their own let them fall into step, and MMAs and exponentials wait for
+    // each other (16 heads of 128, 4096 x 16384: 656 us, this 500 us).
     constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
-    constexpr int kStride = PAIRED ? 2 : 1;  // from one of its tiles to the next
     const bool leader = ptx::elect_one();
     const uint32_t id_s = ptx::make_idesc(1, fmt, kAttnTile);
     const uint32_t id_o =
         ptx::make_idesc(1, fmt, static_cast<uint32_t>((args.D + 15) / 16 * 16)) | ptx::kIdescBMn;
     const int d_steps = (args.D + 15) / 16;
-    const uint32_t q_tile = base + LY::kQ + (PAIRED ? 0 : w) * LY::kTileBytes;
-    const uint64_t q_desc = ptx::sw128_kmajor_desc(q_tile);
+    const uint64_t q_desc = ptx::sw128_kmajor_desc(base + LY::kQ);
     const uint64_t k_desc = ptx::sw128_kmajor_desc(base + LY::kK);
     const uint64_t v_desc = ptx::sw128_mnmajor_desc(base + LY::kV, kAttnBlockBytes);
     const uint32_t q_lo = static_cast<uint32_t>(q_desc), k_lo = static_cast<uint32_t>(k_desc);
     const uint32_t v_lo = static_cast<uint32_t>(v_desc);
     const uint32_t kd_hi = static_cast<uint32_t>(k_desc >> 32);
     const uint32_t v_hi = static_cast<uint32_t>(v_desc >> 32);
-    const uint32_t t_s = tmem + kAttnTile * w, t_o = tmem + 2 * kAttnTile + DP * w;
-    const uint32_t my_q = q_full + (PAIRED ? 0 : 8 * w);
     bool ok = true;
-    uint32_t q_loads = 0, p_turn = 0;
+    uint32_t q_loads[2] = {0, 0}, p_turn[2] = {0, 0};
     auto wait = [&](uint32_t bar, uint32_t parity) {
       const bool got = wait_bar(bar, parity & 1u, wc, DCNV2_DEVERR_TIMEOUT_MMA);
       return ok = __all_sync(0xffffffffu, ok && got);
@@ -381,112 +401,139 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     auto commit = [&](uint32_t bar) {
       if (leader) ptx::tc_commit(bar);
     };
-    auto load_q = [&](int item) {
+    auto load_q = [&](const Item& it, int wg) {
       if (leader) {
-        const Item it = item_at(item);
         const uint32_t rows = args.tile_tokens * args.heads;  // of the box
-        ptx::mbar_arrive_expect_tx(my_q, LY::kBlocks * rows * 128);
+        const uint32_t to = base + LY::kQ + wg * LY::kTileBytes;
+        ptx::mbar_arrive_expect_tx(q_full + 8 * wg, LY::kBlocks * rows * 128);
         for (int x = 0; x < LY::kBlocks; ++x)
-          ptx::tma_load_5d(q_tile + x * kAttnBlockBytes, &tmap_q, x * 64, 0,
-                           it.tok0 + (PAIRED ? 0 : w) * args.tile_tokens, it.g,
-                           it.b * args.q_batch, my_q);
+          ptx::tma_load_5d(to + x * kAttnBlockBytes, &tmap_q, x * 64, 0,
+                           it.tok0 + wg * args.tile_tokens, it.g, it.b * args.q_batch,
+                           q_full + 8 * wg);
       }
-      ++q_loads;
+      ++q_loads[wg];
     };
     // tile i: whether there is one (its K is there then), and of which item
-    int item = item0 - item_step;
-    bool fresh = true, last = true, mine = false;
+    int item = item0;
+    Item it = item_at(item0);
+    bool begun = false, fresh = true, last = true, both = false;
     auto next_tile = [&](int i) {
       if (!wait(k_full + 8 * (i % NS), i / NS)) return false;
       const uint32_t flags = ptx::ld_shared_u32_volatile(base + LY::kFlags + (i % NS) * 4);
       fresh = last;
       last = (flags & kInfoLast) != 0;
-      if (PAIRED) {
-        fresh = item < item0;
-        last = false;
-      }
       if (flags & kTileEnd) return false;
       if (fresh) {
-        item += item_step * static_cast<int>(PAIRED ? 1 : 1 + flags / kTileSkip);
-        mine = rows_of(item_at(item), w) > 0;
+        item += item_step * static_cast<int>(flags / kTileSkip + (begun ? 1 : 0));
+        it = item_at(item);
+        begun = true;
+        both = rows_of(it, 1) > 0;
       }
       return true;
     };
-    auto scores = [&](int i) {  // S from K tile i
+    auto scores = [&](int i, int wg) {  // S of warpgroup wg from K tile i
+      const uint32_t q = q_lo + (PAIRED ? 0 : wg) * (LY::kTileBytes >> 4);
       const uint32_t k = k_lo + (i % NS) * (LY::kTileBytes >> 4);
+      const uint32_t d = tmem + kAttnTile * wg;
       ptx::tc_fence_after();
       if (leader) {
-        ptx::mma_f16_run<false>(t_s, q_lo, kd_hi, k, kd_hi, id_s);
+        ptx::mma_f16_run<false>(d, q, kd_hi, k, kd_hi, id_s);
 #pragma unroll
         for (int x = 1; x < DP / 16; ++x) {
           constexpr uint32_t kBlock = kAttnBlockBytes >> 4;
           const uint32_t off = (x >> 2) * kBlock + (x & 3) * 2;
-          if (x < d_steps) ptx::mma_f16_run<true>(t_s, q_lo + off, kd_hi, k + off, kd_hi, id_s);
+          if (x < d_steps) ptx::mma_f16_run<true>(d, q + off, kd_hi, k + off, kd_hi, id_s);
         }
-        ptx::tc_commit(s_full + 8 * w);
-        ptx::tc_commit(k_empty + 8 * (i % NS));
+        ptx::tc_commit(s_full + 8 * wg);
       }
       __syncwarp();
     };
-    // The scores of a tile are issued right behind the product of the last, whose probabilities they
-    // overwrite: the tensor core runs MMAs in the order of issue.
-    const bool q_shared = PAIRED && w == 1;  // the other issuer loads the one Q
-    int i = PAIRED ? w : 0;
-    bool have = next_tile(i);
-    while (have && ok) {
-      if (!mine) {  // no rows in this item: keep step
-        if (leader) ptx::mbar_arrive(k_empty + 8 * (i % NS));
-        if (!wait(v_full + 8 * (i % NS), i / NS)) break;
-        if (leader) ptx::mbar_arrive(v_empty + 8 * (i % NS));
-        i += kStride;
-        have = next_tile(i);
-        continue;
+    auto product = [&](int i, int wg, bool first) {  // O of warpgroup wg += P V tile i
+      if (!wait(p_ready + 8 * wg, p_turn[wg]++)) return false;
+      ptx::tc_fence_after();
+      const uint32_t v = v_lo + (i % NS) * (LY::kTileBytes >> 4);
+      const uint32_t d = tmem + 2 * kAttnTile + DP * wg, p = tmem + kAttnTile * wg;
+      if (leader) {
+#pragma unroll
+        for (int x = 0; x < kAttnTile / 16; ++x)
+          ptx::mma_f16_ta_run(d, p + 8 * x, v + x * (2048 >> 4), v_hi, id_o,
+                              x > 0 ? 1u : first ? 0u : 1u);
       }
-      // an item begins
-      if (q_shared) ++q_loads;
-      else if (!LY::kOutBeside && !PAIRED && q_loads &&
-               !wait(q_empty + 8 * w, q_loads - 1)) break;  // O of the item ahead has left the place
-      else load_q(item);
-      if (!wait(my_q, q_loads - 1)) break;
-      scores(i);
-      bool first = true, ends = false;
-      while (ok && !ends) {
-        const int cur = i, at = i % NS;
-        i += kStride;
-        ends = last;
-        // Behind an item's end the next tile is looked for after the product: the entries of empty
-        // items in between are read by the softmax only when this item's O is complete.
-        if (!ends) have = next_tile(i);
-        if (PAIRED && !have) ends = true;
-        if (!wait(v_ready + 8 * at, cur / NS)) break;
-        const uint32_t v = v_lo + at * (LY::kTileBytes >> 4);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // O += P V, its halves as the probabilities arrive
-          if (!wait((half ? p_ready : p_half) + 8 * w, p_turn)) break;
-          ptx::tc_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int x = half * 4; x < half * 4 + 4; ++x)
-              ptx::mma_f16_ta_run(t_o, t_s + 8 * x, v + x * (2048 >> 4), v_hi, id_o,
-                                  x > 0 ? 1u : first ? 0u : 1u);
+      __syncwarp();
+      return true;
+    };
+    // A warpgroup's next scores are issued right behind its product, whose probabilities they
+    // overwrite: the tensor core runs MMAs in the order of issue.
+    if constexpr (PAIRED) {
+      int have = 0;       // tiles found
+      bool ended = false;
+      auto more = [&](int upto) {
+        while (ok && !ended && have < upto) {
+          if (next_tile(have)) ++have;
+          else ended = true;
+        }
+        return have >= upto;
+      };
+      load_q(it, 0);
+      wait(q_full, 0);
+      for (int i = 0; i < 2; ++i)
+        if (more(i + 1)) {
+          scores(i, i);
+          commit(k_empty + 8 * (i % NS));
+        }
+      for (int i = 0; ok && i < have; ++i) {
+        const bool next = more(i + 3);
+        if (!wait(v_ready + 8 * (i % NS), i / NS) || !product(i, i & 1, i < 2)) break;
+        if (next) scores(i + 2, i & 1);
+        commit(v_empty + 8 * (i % NS));
+        if (next) commit(k_empty + 8 * ((i + 2) % NS));
+      }
+      commit(o_full);
+      commit(o_full + 8);
+    } else {
+      bool have = next_tile(0);
+      if (have)
+        for (int wg = 0; wg <= both; ++wg) load_q(it, wg);
+      int i = 0;
+      while (have && ok) {  // an item begins: its Q is on its way
+        const bool cur_both = both;
+        for (int wg = 0; wg <= cur_both; ++wg)
+          if (wait(q_full + 8 * wg, q_loads[wg] - 1)) scores(i, wg);
+        commit(k_empty + 8 * (i % NS));
+        bool first = true, ends = false;
+        while (ok && !ends) {
+          const int cur = i++, at = cur % NS;
+          ends = last;
+          // Behind an item's end the next tile is looked for after the products: the entries of empty
+          // items in between are read by the softmax only when this item's O is complete.
+          if (!ends) next_tile(i);
+          if (!wait(v_ready + 8 * at, cur / NS)) break;
+          for (int wg = 0; wg <= cur_both; ++wg) {
+            if (!product(cur, wg, first)) break;
+            if (ends) commit(o_full + 8 * wg);
+            else scores(i, wg);
           }
-          __syncwarp();
+          if (!ok) break;
+          commit(v_empty + 8 * at);
+          if (!ends) commit(k_empty + 8 * (i % NS));
+          first = false;
         }
         if (!ok) break;
-        ++p_turn;
-        first = false;
-        if (!ends) scores(i);
-        else commit(o_full + 8 * w);
-        commit(v_empty + 8 * at);
-        if (!PAIRED && ends) have = next_tile(i);
+        have = next_tile(i);
+        // the next item's Q: this one's scores are done, and where Q is O's way out, O has left it
+        if (have)
+          for (int wg = 0; wg <= both; ++wg) {
+            if (!LY::kOutBeside && q_loads[wg] && !wait(q_empty + 8 * wg, q_loads[wg] - 1)) break;
+            load_q(it, wg);
+          }
       }
     }
-    if (PAIRED && p_turn == 0) commit(o_full + 8 * w);  // no tile of its own
     // what is in flight ends before tensor memory and shared memory are given up
     __syncwarp();
-    commit(base + LY::kDrain + 8 * w);
-    drain_bar(base + LY::kDrain + 8 * w, 0, wc);
-    if (!q_shared && q_loads) drain_bar(my_q, (q_loads - 1) & 1u, wc);
+    commit(base + LY::kDrain);
+    drain_bar(base + LY::kDrain, 0, wc);
+    for (int wg = 0; wg < 2; ++wg)
+      if (q_loads[wg]) drain_bar(q_full + 8 * wg, (q_loads[wg] - 1) & 1u, wc);
   } else if (warp == kAttnFixWarp) {
     // ------------------------------------------------------------ V rows of unkept states
     int n = 0, i = 0;
@@ -536,8 +583,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     uint32_t s_turn = 0, o_turn = 0;
     bool ok = true;
     for (int item = item0; item < args.items && ok; item += item_step) {
-      const Item it = item_at(item);
-      const int n_rows = rows_of(it, w);
+      const int n_rows = rows_of(item_at(item), w);
       const bool mine = n_rows > 0;
       const bool rows_here = (warp & 3) * 32 < n_rows;  // else the warp only keeps step
       const bool live = rl < n_rows;
@@ -557,10 +603,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         if (!ok) break;
         ptx::tc_fence_after();
         if (!rows_here) {
-          if (lane == 0) {
-            ptx::mbar_arrive(p_half + 8 * w);
-            ptx::mbar_arrive(p_ready + 8 * w);
-          }
+          if (lane == 0) ptx::mbar_arrive(p_ready + 8 * w);
           continue;
         }
         uint32_t sc[4][32];
@@ -569,13 +612,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ptx::tmem_wait_ld();
 #pragma unroll
         for (int x = 0; x < 4; ++x) ptx::tmem_ld_use(sc[x]);
-        if ((word[0] & word[1] & word[2] & word[3]) != 0xffffffffu) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 4; ++x)
+          if (word[x] != 0xffffffffu) {
 #pragma unroll
             for (int y = 0; y < 32; ++y)
               if (!((word[x] >> y) & 1u)) sc[x][y] = 0xff800000u;  // -inf
-        }
+          }
         float top[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
@@ -619,18 +662,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int y = 0; y < 16; ++y) {
             const float2 e = ptx::fma2(make_float2(__uint_as_float(sc[x][2 * y]),
                                                    __uint_as_float(sc[x][2 * y + 1])), c2, n2);
-            const float2 p = make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
+            const float2 p = (kAttnFmaPairs >> y) & 1 ? attn_exp2(e)
+                                                      : make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
             sum[y & 1] = ptx::add2(sum[y & 1], p);
             pk[y] = ptx::pack16<BF16>(p.x, p.y);
           }
           ptx::tmem_st_32x32b_x16(t_s + 16 * x, pk);
-          if (x == 1 || x == 3) {
-            ptx::tmem_wait_st();
-            ptx::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive((x == 1 ? p_half : p_ready) + 8 * w);
-          }
         }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(p_ready + 8 * w);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (!mine) continue;
@@ -639,7 +681,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         bool done = ok && wait_bar<kSuspend>(o_full + 8 * w, o_turn & 1u, wc,
                                              DCNV2_DEVERR_TIMEOUT_EPILOGUE);
         if (PAIRED || args.split > 1)
-          done = done && (rows_of(it, w ^ 1) == 0 ||
+          done = done && (rows_of(item_at(item), w ^ 1) == 0 ||
                           wait_bar<kSuspend>(o_full + 8 * (w ^ 1), o_turn & 1u, wc,
                                              DCNV2_DEVERR_TIMEOUT_EPILOGUE));
         ++o_turn;
@@ -654,6 +696,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         // O / sum in the output's type into the swizzled tile that the TMA store reads; the place
         // is free once the last store from it has been read (beside Q), or Q's last scores are done
         // and its last store has been read (over Q)
+        const Item it = item_at(item);
         const uint32_t out = base + LY::kOut + w * LY::kTileBytes;
         const bool storer = (threadIdx.x & 127) == 0;
         if (LY::kOutBeside) {

@@ -443,7 +443,7 @@ dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const void* q, 
 size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc* desc) {
   AttnPlan p;
   if (make_attn_plan(desc, &p) != DCNV2_OK) return 0;
-  return align_up(size_t(p.grid ? p.grid : 1) * sizeof(int), 256);
+  return align_up(size_t(p.grid) * sizeof(int), 256);
 }
 
 dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void* q, const void* k,
@@ -461,8 +461,8 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
     return DCNV2_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(kv_lens) | reinterpret_cast<uintptr_t>(lse)) % 4)
     return DCNV2_ERR_INVALID_ARG;
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 ||
-      workspace_bytes < size_t(p.grid) * sizeof(int))
+  if (p.grid && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 ||
+                 workspace_bytes < size_t(p.grid) * sizeof(int)))
     return DCNV2_ERR_WORKSPACE;
   int dev = 0;
   DevInfo* di = current_device(&dev);
@@ -522,7 +522,7 @@ dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
   AttnPlan p;
   const dcnv2_status s = make_attn_plan(desc, &p);
   if (s != DCNV2_OK) return s;
-  if (!workspace || !code) return DCNV2_ERR_INVALID_ARG;
+  if (!code || (p.grid && !workspace)) return DCNV2_ERR_INVALID_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int32_t bits = 0;
   const int* words = static_cast<const int*>(workspace);

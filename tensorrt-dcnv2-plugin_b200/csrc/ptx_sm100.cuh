@@ -625,6 +625,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // a * b + c of two values at once.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   uint64_t d, x, y, z;

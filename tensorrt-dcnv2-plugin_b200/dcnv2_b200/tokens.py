@@ -31,31 +31,71 @@ def _dtypes():
             torch.bfloat16: int(DType.BF16)}
 
 
+# Calls of these operators take a few microseconds on the GPU, so what depends on the arguments' shapes,
+# strides, types and devices alone (the checks, the desc) is done once for each combination and kept
+# under those values. A tensor is described by:
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
 @contextlib.contextmanager
-def _on(device, stream):
-    """`device` current, and allocations made for `stream` (a raw handle; None: the current one)."""
+def _on(index, stream):
+    """Device `index` current, and allocations made for `stream` (a raw handle; None: the current
+    one); gives the raw handle."""
     import torch
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         if stream is None:
-            yield torch.cuda.current_stream(device).cuda_stream
+            yield torch.cuda.current_stream(index).cuda_stream
         else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream,
+                                                             device=torch.device("cuda", index))):
                 yield stream
 
 
-def _check(what, name, t, dtype, device, ndim):
-    if t.dtype != dtype:
-        raise TypeError(f"{what}: {name} is {t.dtype}, expected {dtype}")
-    if t.dim() != ndim:
-        raise ValueError(f"{what}: {name} has {t.dim()} dimensions, expected {ndim}")
-    if not t.is_cuda or t.device != device:
-        raise ValueError(f"{what}: {name} is not on {device}")
+def _current(index):
+    """The raw handle of the current stream of device `index` if that device is current, else None."""
+    import torch
+    if torch.cuda.current_device() != index:
+        return None
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _check_heads(what, name, t, dtype, device):
-    _check(what, name, t, dtype, device, 4)
-    if t.shape[3] > 1 and t.stride(3) != 1:
+_NOTHING = contextlib.nullcontext()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check(what, name, meta, dtype, index, ndim):
+    shape, _, dt, on = meta
+    if dt != dtype:
+        raise TypeError(f"{what}: {name} is {dt}, expected {dtype}")
+    if len(shape) != ndim:
+        raise ValueError(f"{what}: {name} has {len(shape)} dimensions, expected {ndim}")
+    if on < 0 or on != index:
+        raise ValueError(f"{what}: {name} is not on cuda:{index}")
+
+
+def _check_heads(what, name, meta, dtype, index):
+    _check(what, name, meta, dtype, index, 4)
+    if meta[0][3] > 1 and meta[1][3] != 1:
         raise ValueError(f"{what}: the elements of a head of {name} are not contiguous")
+
+
+def _contiguous(shape, strides):
+    step = 1
+    for n, st in zip(reversed(shape), reversed(strides)):
+        if n > 1 and st != step:
+            return 0 in shape
+        step *= n
+    return True
+
+
+def _packed(shape):
+    """Batch, token and head strides of a contiguous tensor."""
+    _, t, h, d = shape
+    return t * h * d, h * d, d
 
 
 def rotary_axes(rotary_dim: int, sections: Sequence[int], base: float = 10000.0,
@@ -99,15 +139,67 @@ def level_positions(sizes: Sequence[Sequence[int]], device="cuda"):
 
 
 @functools.lru_cache(maxsize=1024)
-def _rotary_desc(batch, tokens, q_heads, k_heads, head_dim, rotary_dim, axes, dtype, norm,
-                 interleaved, eps, pair_axis, strides, pos_batch_stride):
-    d = RotaryDesc(batch, tokens, q_heads, k_heads, head_dim, rotary_dim, axes, dtype, norm,
-                   interleaved, eps)
+def _rotary_plan(q, k, q_out, k_out, positions, freqs, q_weight, k_weight, pair_axis, norm, eps,
+                 interleaved):
+    """Checks the metas; (desc, device index, whether there is nothing to do)."""
+    import torch
+    what = "dcnv2_qk_norm_rotary"
+    x = q or k
+    if x is None:
+        raise ValueError(f"{what}: q or k is needed")
+    shape, _, dt, index = x
+    if dt not in _dtypes():
+        raise TypeError(f"{what}: unsupported dtype {dt}")
+    if norm not in (None, "rms"):
+        raise ValueError(f"{what}: norm is None or 'rms'")
+    for name, t, o, w in (("q", q, q_out, q_weight), ("k", k, k_out, k_weight)):
+        if t is None:
+            if o is not None or w is not None:
+                raise ValueError(f"{what}: {name}_out or {name}_weight without {name}")
+            continue
+        _check_heads(what, name, t, dt, index)
+        if (t[0][0], t[0][1], t[0][3]) != (shape[0], shape[1], shape[3]):
+            raise ValueError(f"{what}: q and k differ in batch, tokens or head_dim")
+        if o is not None:
+            _check_heads(what, f"{name}_out", o, dt, index)
+            if o[0] != t[0]:
+                raise ValueError(f"{what}: {name}_out has another shape than {name}")
+        if w is not None:
+            _check(what, f"{name}_weight", w, dt, index, 1)
+            if w[0][0] != shape[3] or not _contiguous(w[0], w[1]):
+                raise ValueError(f"{what}: {name}_weight is not a contiguous [{shape[3]}]")
+            if norm is None:
+                raise ValueError(f"{what}: {name}_weight without norm='rms'")
+    B, T, _, D = shape
+    pairs, axes, pos_sb = 0, 1, 0
+    if freqs is not None:
+        pairs = len(pair_axis)
+        _check(what, "freqs", freqs, torch.float32, index, 1)
+        if freqs[0][0] != pairs or not _contiguous(freqs[0], freqs[1]) or 2 * pairs > D or \
+                pairs > 128:
+            raise ValueError(f"{what}: freqs and pair_axis give one value for each of at most "
+                             f"{min(D // 2, 128)} rotated pairs")
+        if positions is None:
+            raise ValueError(f"{what}: rotation needs positions")
+        if len(positions[0]) == 2:
+            positions = ((1,) + tuple(positions[0]), (0,) + tuple(positions[1])) + positions[2:]
+        _check(what, "positions", positions, torch.int32, index, 3)
+        (n, tokens, axes), strides = positions[0], positions[1]
+        if n not in (1, B) or tokens != T or not _contiguous(positions[0], strides):
+            raise ValueError(f"{what}: positions are not a contiguous [{B} or 1, {T}, axes]")
+        pos_sb = T * axes if n > 1 else 0
+    elif positions is not None or len(pair_axis):
+        raise ValueError(f"{what}: positions or pair_axis without freqs")
+    d = RotaryDesc(B, T, q[0][2] if q else 0, k[0][2] if k else 0, D, 2 * pairs, axes,
+                   _dtypes()[dt], int(Norm.RMS if norm else Norm.NONE), int(interleaved), eps)
     ctypes.memmove(d.pair_axis, pair_axis, len(pair_axis))
-    for field, st in zip((d.q_stride, d.k_stride, d.q_out_stride, d.k_out_stride), strides):
-        field[:] = st
-    d.pos_batch_stride = pos_batch_stride
-    return d
+    for t, o, field, out_field in ((q, q_out, d.q_stride, d.q_out_stride),
+                                   (k, k_out, d.k_stride, d.k_out_stride)):
+        if t is not None:
+            field[:] = t[1][:3]
+            out_field[:] = o[1][:3] if o is not None else _packed(t[0])
+    d.pos_batch_stride = pos_sb
+    return d, index, 0 in (B, T, D) or not (d.q_heads or d.k_heads)
 
 
 def dcnv2_qk_norm_rotary(q, k=None, positions=None, freqs=None, pair_axis=b"", q_weight=None,
@@ -125,93 +217,66 @@ def dcnv2_qk_norm_rotary(q, k=None, positions=None, freqs=None, pair_axis=b"", q
     q_out, k_out  outputs; q and k themselves rotate in place
     Returns contiguous tensors unless outputs are given; None stands for an absent one."""
     import torch
-    what = "dcnv2_qk_norm_rotary"
-    x = q if q is not None else k
-    if x is None:
-        raise ValueError(f"{what}: q or k is needed")
-    if x.dtype not in _dtypes():
-        raise TypeError(f"{what}: unsupported dtype {x.dtype}")
-    if norm not in (None, "rms"):
-        raise ValueError(f"{what}: norm is None or 'rms'")
-    dt, dev = x.dtype, x.device
-    B, T, D = x.shape[0], x.shape[1], x.shape[-1]
-    outs = []
-    for name, t, o, w in (("q", q, q_out, q_weight), ("k", k, k_out, k_weight)):
-        if t is None:
-            if o is not None or w is not None:
-                raise ValueError(f"{what}: {name}_out or {name}_weight without {name}")
-            continue
-        _check_heads(what, name, t, dt, dev)
-        if (t.shape[0], t.shape[1], t.shape[3]) != (B, T, D):
-            raise ValueError(f"{what}: q and k differ in batch, tokens or head_dim")
-        if o is not None:
-            _check_heads(what, f"{name}_out", o, dt, dev)
-            if o.shape != t.shape:
-                raise ValueError(f"{what}: {name}_out has another shape than {name}")
-        if w is not None:
-            _check(what, f"{name}_weight", w, dt, dev, 1)
-            if w.shape[0] != D or not w.is_contiguous():
-                raise ValueError(f"{what}: {name}_weight is not a contiguous [{D}]")
-            if norm is None:
-                raise ValueError(f"{what}: {name}_weight without norm='rms'")
-    pairs, axes, pos_sb = 0, 1, 0
-    if freqs is not None:
-        pair_axis = bytes(pair_axis)
-        pairs = len(pair_axis)
-        _check(what, "freqs", freqs, torch.float32, dev, 1)
-        if freqs.shape[0] != pairs or not freqs.is_contiguous() or 2 * pairs > D or pairs > 128:
-            raise ValueError(f"{what}: freqs and pair_axis give one value for each of at most "
-                             f"{min(D // 2, 128)} rotated pairs")
-        if positions is None:
-            raise ValueError(f"{what}: rotation needs positions")
-        if positions.dim() == 2:
-            positions = positions[None]
-        _check(what, "positions", positions, torch.int32, dev, 3)
-        if positions.shape[0] not in (1, B) or positions.shape[1] != T or \
-                not positions.is_contiguous():
-            raise ValueError(f"{what}: positions are not a contiguous [{B} or 1, {T}, axes]")
-        axes = positions.shape[2]
-        pos_sb = T * axes if positions.shape[0] > 1 else 0
-    elif positions is not None or len(pair_axis):
-        raise ValueError(f"{what}: positions or pair_axis without freqs")
-    same = stream is None and dev.index == torch.cuda.current_device()
-    with contextlib.nullcontext() if same else _on(dev, stream) as st:
-        if same:
-            st = torch.cuda.current_stream().cuda_stream
+    desc, index, nothing = _rotary_plan(
+        _meta(q), _meta(k), _meta(q_out), _meta(k_out), _meta(positions), _meta(freqs),
+        _meta(q_weight), _meta(k_weight), bytes(pair_axis), norm, float(eps), bool(interleaved))
+    st = _current(index) if stream is None else None
+    with _NOTHING if st is not None else _on(index, stream) as other:
         if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=dev)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if k is not None and k_out is None:
-            k_out = torch.empty(k.shape, dtype=dt, device=dev)
-        strides = tuple(t.stride()[:3] if t is not None else (0, 0, 0)
-                        for t in (q, k, q_out, k_out))
-        desc = _rotary_desc(B, T, q.shape[2] if q is not None else 0,
-                            k.shape[2] if k is not None else 0, D, 2 * pairs, axes,
-                            _dtypes()[dt], int(Norm.RMS if norm else Norm.NONE), int(interleaved),
-                            float(eps), pair_axis, strides, pos_sb)
-        if x.numel() == 0 and (k is None or k.numel() == 0):
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        if nothing:
             return q_out, k_out
         rc = lib.dcnv2_qk_norm_rotary(
-            ctypes.byref(desc), *(t.data_ptr() if t is not None else None for t in (
-                q, k, positions, freqs, q_weight, k_weight, q_out, k_out)), st)
+            ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(positions), _ptr(freqs), _ptr(q_weight),
+            _ptr(k_weight), _ptr(q_out), _ptr(k_out), other if st is None else st)
     if rc != Status.OK:
-        raise DCNv2Error(rc, what)
+        raise DCNv2Error(rc, "dcnv2_qk_norm_rotary")
     return q_out, k_out
 
 
 @functools.lru_cache(maxsize=1024)
-def _attention_desc(batch, q_tokens, kv_tokens, q_heads, kv_heads, head_dim, dtype, scale, strides,
-                    mask_batch_stride):
-    """The desc and its workspace size."""
-    d = AttentionDesc(batch, q_tokens, kv_tokens, q_heads, kv_heads, head_dim, dtype, scale)
-    for field, st in zip((d.q_stride, d.k_stride, d.v_stride, d.out_stride), strides):
-        field[:] = st
-    d.mask_batch_stride = mask_batch_stride
-    return d, int(lib.dcnv2_cross_attention_workspace_size(ctypes.byref(d)))
-
-
-def _legal_strides(t):
-    """Batch, token and head strides; of a dimension that takes no step, 0."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride(), t.shape[:3]))
+def _attention_plan(q, k, v, out, kv_lens, key_mask, scale):
+    """Checks the metas; (desc, workspace bytes, device index, shape of lse, whether there is nothing
+    to do)."""
+    import torch
+    what = "dcnv2_cross_attention"
+    (B, L, H, D), _, dt, index = q if len(q[0]) == 4 else ((0, 0, 0, 0),) + q[1:]
+    if dt not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"{what}: unsupported dtype {dt}")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check_heads(what, name, t, dt, index)
+    _, S, G, _ = k[0]
+    if k[0][0] != B or k[0][3] != D or v[0] != k[0]:
+        raise ValueError(f"{what}: k and v are not [{B}, kv_tokens, kv_heads, {D}]")
+    if out is not None:
+        _check_heads(what, "out", out, dt, index)
+        if out[0] != q[0]:
+            raise ValueError(f"{what}: out has another shape than q")
+    if kv_lens is not None:
+        _check(what, "kv_lens", kv_lens, torch.int32, index, 1)
+        if kv_lens[0][0] != B or not _contiguous(kv_lens[0], kv_lens[1]):
+            raise ValueError(f"{what}: kv_lens is not a contiguous [{B}]")
+    mask_sb = 0
+    if key_mask is not None:
+        if key_mask[2] not in (torch.bool, torch.uint8):
+            raise TypeError(f"{what}: key_mask is bool or uint8")
+        _check(what, "key_mask", key_mask, key_mask[2], index, 2)
+        if key_mask[0][0] not in (1, B) or key_mask[0][1] != S or (S > 1 and key_mask[1][1] != 1):
+            raise ValueError(f"{what}: key_mask is not [{B} or 1, {S}] with contiguous rows")
+        mask_sb = key_mask[1][0] if key_mask[0][0] > 1 else 0
+    if scale is None:
+        scale = 1.0 / math.sqrt(D) if D else 1.0
+    d = AttentionDesc(B, L, S, H, G, D, _dtypes()[dt], scale)
+    for field, shape, strides in ((d.q_stride, q[0], q[1]), (d.k_stride, k[0], k[1]),
+                                  (d.v_stride, v[0], v[1]),
+                                  (d.out_stride, q[0], out[1] if out else _packed(q[0]))):
+        # of a dimension that takes no step, 0
+        field[:] = tuple(st if n > 1 else 0 for st, n in zip(strides, shape[:3]))
+    d.mask_batch_stride = mask_sb
+    nothing = 0 in (B, L, H, D)
+    return (d, 0 if nothing else capi.attention_workspace_size(d), index, (B, H, L), nothing)
 
 
 def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
@@ -225,60 +290,31 @@ def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
     kv_lens    int32 [batch]: kept states per sequence; None keeps all
     key_mask   bool or uint8 [batch or 1, kv_tokens]: states kept (pixels of padded images)
     scale      of the scores; None: 1 / sqrt(head_dim)
-    workspace  uint8 CUDA tensor of at least dcnv2_cross_attention_workspace_size bytes (allocated
-               when absent or too small); not shared by calls that may overlap
+    workspace  CUDA tensor of at least dcnv2_cross_attention_workspace_size bytes (allocated when
+               absent or too small); not shared by calls that may overlap
     All tensors: any strides that are multiples of 8 elements, contiguous heads, 16-byte aligned;
     head_dim a multiple of 8, at most 128. A sequence without kept states gives zeros. Returns out
     [batch, q_tokens, q_heads, head_dim], or (out, lse) with lse fp32 [batch, q_heads, q_tokens]."""
     import torch
-    what = "dcnv2_cross_attention"
-    dt, dev = q.dtype, q.device
-    if dt not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"{what}: unsupported dtype {dt}")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check_heads(what, name, t, dt, dev)
-    B, L, H, D = q.shape
-    S, G = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape:
-        raise ValueError(f"{what}: k and v are not [{B}, kv_tokens, kv_heads, {D}]")
-    if out is not None:
-        _check_heads(what, "out", out, dt, dev)
-        if out.shape != q.shape:
-            raise ValueError(f"{what}: out has another shape than q")
-    if kv_lens is not None:
-        _check(what, "kv_lens", kv_lens, torch.int32, dev, 1)
-        if kv_lens.shape[0] != B or not kv_lens.is_contiguous():
-            raise ValueError(f"{what}: kv_lens is not a contiguous [{B}]")
-    mask_sb = 0
-    if key_mask is not None:
-        if key_mask.dtype not in (torch.bool, torch.uint8):
-            raise TypeError(f"{what}: key_mask is bool or uint8")
-        _check(what, "key_mask", key_mask, key_mask.dtype, dev, 2)
-        if key_mask.shape[0] not in (1, B) or key_mask.shape[1] != S or \
-                (S > 1 and key_mask.stride(1) != 1):
-            raise ValueError(f"{what}: key_mask is not [{B} or 1, {S}] with contiguous rows")
-        mask_sb = key_mask.stride(0) if key_mask.shape[0] > 1 else 0
-    if scale is None:
-        scale = 1.0 / math.sqrt(D) if D else 1.0
-    if workspace is not None and (not workspace.is_cuda or workspace.device != dev):
-        raise ValueError(f"{what}: workspace is not on {dev}")
-    same = stream is None and dev.index == torch.cuda.current_device()
-    with contextlib.nullcontext() if same else _on(dev, stream) as st:
-        if same:
-            st = torch.cuda.current_stream().cuda_stream
+    desc, ws_bytes, index, lse_shape, nothing = _attention_plan(
+        _meta(q), _meta(k), _meta(v), _meta(out), _meta(kv_lens), _meta(key_mask),
+        None if scale is None else float(scale))
+    if workspace is not None and workspace.get_device() != index:
+        raise ValueError(f"dcnv2_cross_attention: workspace is not on cuda:{index}")
+    st = _current(index) if stream is None else None
+    with _NOTHING if st is not None else _on(index, stream) as other:
         if out is None:
-            out = torch.empty(q.shape, dtype=dt, device=dev)
-        lse = torch.empty((B, H, L), dtype=torch.float32, device=dev) if return_lse else None
-        if out.numel() == 0:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device) if return_lse else None
+        if nothing:
             return (out, lse) if return_lse else out
-        desc, ws_bytes = _attention_desc(
-            B, L, S, H, G, D, _dtypes()[dt], float(scale),
-            tuple(_legal_strides(t) for t in (q, k, v, out)), mask_sb)
-        if workspace is None or workspace.numel() < ws_bytes:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        if workspace is None or workspace.nbytes < ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes \
+                else None
         rc = lib.dcnv2_cross_attention(
-            ctypes.byref(desc), *(t.data_ptr() if t is not None else None for t in (
-                q, k, v, kv_lens, key_mask, out, lse, workspace)), workspace.numel(), st)
+            ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(kv_lens), _ptr(key_mask),
+            _ptr(out), _ptr(lse), _ptr(workspace), workspace.nbytes if workspace is not None else 0,
+            other if st is None else st)
     if rc != Status.OK:
-        raise DCNv2Error(rc, what)
+        raise DCNv2Error(rc, "dcnv2_cross_attention")
     return (out, lse) if return_lse else out
