@@ -109,7 +109,9 @@ struct AttnLayout {
   static constexpr uint32_t kPart = kK;
   static constexpr uint32_t kPartBytes = kAttnTile * DP * 4;
   static_assert(2 * kPartBytes <= 2 * kStages * kTileBytes, "parts fit over K and V");
-  static_assert(2 * kAttnTile * 8 <= kK, "statistics fit over Q");
+  static_assert(2 * kAttnTile * 8 + (PAIRED ? kAttnTile : 2 * kAttnTile) *
+                                        (PAIRED ? 2 : 1) * kAttnMaxSplit * 4 <= kK,
+                "statistics and shares fit over Q");
 };
 template <int DP, bool PAIRED>
 constexpr size_t attn_smem_bytes() {
@@ -773,66 +775,72 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       ptx::tc_fence_before();
       ptx::cluster_sync();
       {
-        // an item is 8 elements of a row; the CTAs of the cluster take turns
+        // This CTA finishes a block of the item's rows: first every row's share of each part (part y: of
+        // CTA y, or of warpgroup y % 2 of CTA y / 2), then 4 elements per thread, the loads of all
+        // parts in flight at once and a warp's in one row.
         constexpr int MP = PAIRED ? 2 * kAttnMaxSplit : kAttnMaxSplit;
         const Item it = item_at(item0);
-        const int chunks = args.D / 8, parts = PAIRED ? 2 * args.split : args.split;
+        const int parts = PAIRED ? 2 * args.split : args.split;
         const int rows0 = rows_of(it, 0), n_rows = rows0 + (PAIRED ? 0 : rows_of(it, 1));
-        for (int x = rank * 256 + static_cast<int>(threadIdx.x); x < n_rows * chunks;
-             x += args.split * 256) {
-          const int r = x / chunks, ch = x - r * chunks;
-          const int rw = r < rows0 ? 0 : 1, rt = r - rw * rows0;  // warpgroup's tile, row of it
-          // part y: of CTA y, or of warpgroup y % 2 of CTA y / 2
-          auto cta = [&](int y) { return PAIRED ? y >> 1 : y; };
-          auto wg = [&](int y) { return PAIRED ? y & 1 : rw; };
-          float2 ml[MP];  // loads of all parts are in flight at once
-          float top = -INFINITY;
-  #pragma unroll
+        const int block = (n_rows + args.split - 1) / args.split;
+        const int r0 = rank * block, r1 = min(n_rows, r0 + block);
+        auto cta = [&](int y) { return PAIRED ? y >> 1 : y; };
+        auto wg = [&](int y, int r) { return PAIRED ? y & 1 : r < rows0 ? 0 : 1; };
+        auto tile_row = [&](int r) { return r < rows0 ? r : r - rows0; };
+        // behind the statistics that the other CTAs read: [row of the block][part] factors
+        float* share = reinterpret_cast<float*>(smem + LY::kQ + 2 * kAttnTile * 8);
+        for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += 256) {
+          float2 ml[MP];
+          float top = -INFINITY, total = 0.f;
+#pragma unroll
           for (int y = 0; y < MP; ++y)
             if (y < parts)
-              ml[y] = ptx::ld_cluster_f2(
-                  ptx::mapa_shared(base + LY::kQ + (wg(y) * kAttnTile + rt) * 8, cta(y)));
-  #pragma unroll
+              ml[y] = ptx::ld_cluster_f2(ptx::mapa_shared(
+                  base + LY::kQ + (wg(y, r) * kAttnTile + tile_row(r)) * 8, cta(y)));
+#pragma unroll
           for (int y = 0; y < MP; ++y)
             if (y < parts) top = fmaxf(top, ml[y].x);
-          float total = 0.f, acc[8] = {};
-  #pragma unroll
-          for (int y0 = 0; y0 < MP; y0 += 4) {
-            float4 lo[4], hi[4];
-  #pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (y0 + y < parts) {
-                const uint32_t at = base + LY::kPart + wg(y0 + y) * LY::kPartBytes;
-                lo[y] = ptx::ld_cluster_f4(
-                    ptx::mapa_shared(at + attn_part_at<DP>(rt, 2 * ch), cta(y0 + y)));
-                hi[y] = ptx::ld_cluster_f4(
-                    ptx::mapa_shared(at + attn_part_at<DP>(rt, 2 * ch + 1), cta(y0 + y)));
-              }
-  #pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (y0 + y < parts) {
-                const float2 q = ml[y0 + y];
-                const float f = q.x == top ? 1.f : ptx::ex2((q.x - top) * c);
-                total = fmaf(q.y, f, total);
-                acc[0] = fmaf(lo[y].x, f, acc[0]); acc[1] = fmaf(lo[y].y, f, acc[1]);
-                acc[2] = fmaf(lo[y].z, f, acc[2]); acc[3] = fmaf(lo[y].w, f, acc[3]);
-                acc[4] = fmaf(hi[y].x, f, acc[4]); acc[5] = fmaf(hi[y].y, f, acc[5]);
-                acc[6] = fmaf(hi[y].z, f, acc[6]); acc[7] = fmaf(hi[y].w, f, acc[7]);
-              }
-          }
-          const int tok = it.tok0 + rw * args.tile_tokens + rt / args.heads;
-          const int h = it.g * args.heads + rt % args.heads;
+#pragma unroll
+          for (int y = 0; y < MP; ++y)
+            if (y < parts) {
+              ml[y].x = ml[y].x == top ? 1.f : ptx::ex2((ml[y].x - top) * c);
+              total = fmaf(ml[y].y, ml[y].x, total);
+            }
           const float inv = total == 0.f ? 0.f : 1.f / total;
-          uint32_t pk[4];
-  #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            pk[y] = ptx::pack16<BF16>(acc[2 * y] * inv, acc[2 * y + 1] * inv);
-          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(args.out) + it.b * args.out_sb +
-                                    tok * args.out_st + h * args.out_sh + ch * 8) =
-              make_uint4(pk[0], pk[1], pk[2], pk[3]);
-          if (args.lse && ch == 0)
+#pragma unroll
+          for (int y = 0; y < MP; ++y)
+            if (y < parts) share[(r - r0) * MP + y] = ml[y].x * inv;
+          if (args.lse) {
+            const int tr = tile_row(r);
+            const int tok = it.tok0 + (r < rows0 ? 0 : args.tile_tokens) + tr / args.heads;
+            const int h = it.g * args.heads + tr % args.heads;
             args.lse[(static_cast<int64_t>(it.b) * args.H + h) * args.L + tok] =
                 total == 0.f ? -INFINITY : kLn2 * (top * c - shift + log2f(total));
+          }
+        }
+        ptx::named_barrier(1, 256);
+        const int quads = args.D / 4;
+        for (int x = threadIdx.x; x < (r1 - r0) * quads; x += 256) {
+          const int rb = x / quads, r = r0 + rb, ch = x - rb * quads, tr = tile_row(r);
+          float4 o[MP];
+#pragma unroll
+          for (int y = 0; y < MP; ++y)
+            if (y < parts)
+              o[y] = ptx::ld_cluster_f4(ptx::mapa_shared(
+                  base + LY::kPart + wg(y, r) * LY::kPartBytes + attn_part_at<DP>(tr, ch), cta(y)));
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int y = 0; y < MP; ++y)
+            if (y < parts) {
+              const float f = share[rb * MP + y];
+              acc.x = fmaf(o[y].x, f, acc.x); acc.y = fmaf(o[y].y, f, acc.y);
+              acc.z = fmaf(o[y].z, f, acc.z); acc.w = fmaf(o[y].w, f, acc.w);
+            }
+          const int tok = it.tok0 + (r < rows0 ? 0 : args.tile_tokens) + tr / args.heads;
+          const int h = it.g * args.heads + tr % args.heads;
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(args.out) + it.b * args.out_sb +
+                                    tok * args.out_st + h * args.out_sh + ch * 4) =
+              make_uint2(ptx::pack16<BF16>(acc.x, acc.y), ptx::pack16<BF16>(acc.z, acc.w));
         }
       }
       ptx::cluster_sync();  // the parts stay until every CTA has read them

@@ -171,6 +171,27 @@ struct AttnPlan {
 
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
 
+// CTAs of a cluster that split the states of one item, from the time of the whole in units of a state
+// tile (about 2 us: its MMAs and exponentials for both warpgroups): waves of clusters * (tiles of a
+// CTA + start + join). An item that is not split costs no join, and one start for all items of its
+// CTA. (18 items of 8 tiles, split 8: 15 of the clusters run at once, 26 us; split 4: 13 us.)
+int attn_split(int64_t items, int64_t tiles) {
+  // clusters of 1, 2, ... CTAs that run at once with one CTA per SM, as the GPCs of 148 SMs allow
+  static constexpr int kResident[kAttnMaxSplit + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+  constexpr double kStart = 1.5, kJoin = 1.0;
+  int best = 1;
+  double least = static_cast<double>(cdiv(items, kPlanSms)) * tiles + kStart;
+  for (int s = 2; s <= kAttnMaxSplit && s <= tiles; ++s) {
+    const double t = static_cast<double>(cdiv(items, kResident[s])) *
+                     (static_cast<double>(cdiv(tiles, s)) + kStart + kJoin);
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
 dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   if (!d) return DCNV2_ERR_INVALID_ARG;
   if (d->dtype != DCNV2_HALF && d->dtype != DCNV2_BF16) return DCNV2_ERR_UNSUPPORTED;
@@ -212,11 +233,7 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   const int64_t groups = int64_t(d->kv_heads) * p->kv_parts;
   if (groups > INT_MAX || int64_t(d->batch) * groups > INT_MAX) return DCNV2_ERR_INVALID_ARG;
   const int64_t ctas = int64_t(d->batch) * groups * p->row_tiles;
-  // Split the states over as many CTAs as still run at once, each with a tile at least.
-  p->split = 1;
-  while (p->split < kAttnMaxSplit && ctas * p->split * 2 <= kPlanSms &&
-         cdiv(d->kv_tokens, kAttnTile) >= int64_t(p->split) * 2 * (p->paired ? 2 : 1))
-    p->split *= 2;
+  p->split = attn_split(ctas, cdiv(d->kv_tokens, kAttnTile * (p->paired ? 2 : 1)));
   if (ctas * p->split > INT_MAX) return DCNV2_ERR_INVALID_ARG;
   p->items = static_cast<int>(ctas);
   // items that are not split or joined are taken in turn by one CTA per SM
