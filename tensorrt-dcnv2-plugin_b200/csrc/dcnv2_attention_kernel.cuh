@@ -38,9 +38,6 @@
 #include <stdint.h>
 
 #include "../../include/dcnv2.h"
-#ifndef FMAP
-#define FMAP 0
-#endif
 #include "dcnv2_wait.cuh"
 #include "ptx_sm100.cuh"
 
@@ -52,7 +49,6 @@ constexpr int kAttnProducerWarp = 8, kAttnMmaWarp = 9, kAttnFixWarp = 10;  // (1
 constexpr uint32_t kAttnBlockBytes = kAttnTile * 128;  // 128 rows of one 128-byte swizzle block
 constexpr int kAttnMaxSplit = 8;               // CTAs of a cluster (portable size)
 constexpr float kAttnLazy = 8.f;               // log2 of the growth that rescales
-constexpr uint32_t kAttnFmaPairs = FMAP;     // of 16 pairs of exponentials, those on the FMA units
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnTensor {
@@ -123,27 +119,6 @@ constexpr size_t attn_smem_bytes() {
 template <int DP>
 __device__ __forceinline__ uint32_t attn_part_at(int r, int c) {
   return static_cast<uint32_t>(r) * (DP * 4) + (static_cast<uint32_t>(c ^ (r & 7)) << 4);
-}
-
-// 2^x of two values on the FMA units, for the share of the exponentials that the special-function
-// units (16 per clock and SM) have no time for: x = n + f with n the nearest integer (taken from the
-// low bits of x + 1.5 * 2^23), 2^f by the polynomial of degree 5 whose relative error on [-1/2, 1/2] is
-// least (7.5e-8, found by Remez exchange), n added to the exponent. x is at most 15 here; below -126
-// the result is 2^-126 and less than 10^-37 of the row's largest.
-__device__ __forceinline__ float2 attn_exp2(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = ptx::add2(x, make_float2(12582912.f, 12582912.f));
-  const float2 f =
-      ptx::fma2(ptx::add2(t, make_float2(-12582912.f, -12582912.f)), make_float2(-1.f, -1.f), x);
-  float2 p = ptx::fma2(f, make_float2(0.0013276472454890609f, 0.0013276472454890609f),
-                       make_float2(0.009675540961325169f, 0.009675540961325169f));
-  p = ptx::fma2(p, f, make_float2(0.05550713092088699f, 0.05550713092088699f));
-  p = ptx::fma2(p, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
-  p = ptx::fma2(p, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
-  p = ptx::fma2(p, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 
 // What the producer says of a tile, beside its kept-state words.
@@ -261,9 +236,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     return true;
   };
 
-  // 384 threads x 168 registers at launch cover 256 x 208 + 128 x 80
+  // 384 threads x 168 registers at launch cover 256 x 192 + 128 x 120
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
   if (warp == kAttnProducerWarp) {
     // ------------------------------------------------------------ producer
     int n = 0, i = 0;                    // ring entries, tiles
@@ -576,7 +551,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     ptx::cluster_sync();
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ------------------------------------------------------------ softmax
     const int rl = (warp & 3) * 32 + lane;  // row of the tile = tensor-memory lane
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
@@ -624,17 +599,15 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         float top[8];
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-          top[x] = __uint_as_float(sc[x >> 1][(x & 1) * 16]);
+          const uint32_t* q = &sc[x >> 1][(x & 1) * 16];
+          top[x] = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+#pragma unroll
+          for (int y = 2; y < 16; y += 2)
+            top[x] = ptx::max3(top[x], __uint_as_float(q[y]), __uint_as_float(q[y + 1]));
         }
-#pragma unroll
-        for (int y = 1; y < 16; ++y)
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-            top[x] = fmaxf(top[x], __uint_as_float(sc[x >> 1][(x & 1) * 16 + y]));
-#pragma unroll
-        for (int x = 4; x > 0; x >>= 1)
-#pragma unroll
-          for (int y = 0; y < x; ++y) top[y] = fmaxf(top[y], top[y + x]);
+        top[0] = ptx::max3(top[0], top[1], top[2]);
+        top[3] = ptx::max3(top[3], top[4], top[5]);
+        top[0] = fmaxf(ptx::max3(top[0], top[3], top[6]), top[7]);
         const float m = fmaxf(m_ref, top[0]);
         // (-inf) - (-inf) is NaN, which is not greater
         if (__any_sync(0xffffffffu, (m - m_ref) * c > kAttnLazy)) {
@@ -664,8 +637,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int y = 0; y < 16; ++y) {
             const float2 e = ptx::fma2(make_float2(__uint_as_float(sc[x][2 * y]),
                                                    __uint_as_float(sc[x][2 * y + 1])), c2, n2);
-            const float2 p = (kAttnFmaPairs >> y) & 1 ? attn_exp2(e)
-                                                      : make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
+            const float2 p = make_float2(ptx::ex2(e.x), ptx::ex2(e.y));
             sum[y & 1] = ptx::add2(sum[y & 1], p);
             pk[y] = ptx::pack16<BF16>(p.x, p.y);
           }
