@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(kStepThreads)
     }
   const float c = args.scale * kLog2e;
   const float shift = BF16 ? 0.f : 7.f;  // as in the tiled kernel
+  const bool upper = args.rows > 8;      // rows 8 to 15 are in use
   float m_ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   float o[OT][4];
 #pragma unroll
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(kStepThreads)
     }
     // ((-inf) - (-inf) is NaN, which is not greater)
     if (__any_sync(0xffffffffu, (top[0] - m_ref[0]) * c > kAttnLazy ||
-                                    (top[1] - m_ref[1]) * c > kAttnLazy)) {
+                                    (upper && (top[1] - m_ref[1]) * c > kAttnLazy))) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float m = fmaxf(m_ref[r], top[r]);
@@ -264,6 +265,11 @@ __global__ void __launch_bounds__(kStepThreads)
     }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
+      if (r == 1 && !upper) {  // no such rows: no exponentials
+#pragma unroll
+        for (int x = 0; x < NT; ++x) s[x][2] = s[x][3] = 0.f;
+        continue;
+      }
       const float neg = (m_ref[r] == -INFINITY ? 0.f : -m_ref[r] * c) + shift;
       float sum[2] = {0.f, 0.f};
 #pragma unroll

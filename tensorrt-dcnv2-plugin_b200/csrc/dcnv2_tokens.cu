@@ -340,12 +340,12 @@ dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPl
 // CTAs of a cluster that split the states of one (sequence, kv head): as few as give every SM a CTA,
 // with a chunk for each of their warps. One CTA draws at most about 50 GB/s, so that fewer CTAs than
 // SMs leave bandwidth unused, while more cost their start and end again (32 x 8 heads of 32, 5456
-// states: 256 CTAs 32 us, 512 36 us, 1024 45 us; 8 kv heads of 128, 5456 states: 64 CTAs 12.9 us, 128
-// 10.7 us). Lengths of their own leave SMs idle behind the short sequences; twice the CTAs even that
-// out (8 x 8 heads of 128, up to 60001 states: 128 CTAs 245 us, 512 210 us).
+// states: 256 CTAs 32 us, 512 36 us, 1024 44 us; 8 kv heads of 128, 5456 states: 64 CTAs 12.9 us, 128
+// 10.9 us). Lengths of their own leave SMs idle behind the short sequences; four times the CTAs even
+// that out (8 x 8 heads of 128, up to 60001 states: 128 CTAs 240 us, 512 208 us, 1024 200 us).
 int step_split(int64_t units, const AttnStepArgs& a, int sm_count) {
   const int keys = a.D > 64 ? 16 : a.D > 32 ? 32 : 64;
-  const int64_t want = int64_t(sm_count) * (a.kv_lens ? 2 : 1);
+  const int64_t want = int64_t(sm_count) * (a.kv_lens ? 4 : 1);
   int split = 1;
   while (split < kStepMaxSplit && units * split < want &&
          cdiv(a.S, keys) >= int64_t(split) * 2 * kStepWarps)
