@@ -196,7 +196,7 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   if (!d) return DCNV2_ERR_INVALID_ARG;
   if (d->dtype != DCNV2_HALF && d->dtype != DCNV2_BF16) return DCNV2_ERR_UNSUPPORTED;
   if (d->batch < 0 || d->q_tokens < 0 || d->kv_tokens < 0 || d->q_heads < 1 || d->kv_heads < 1 ||
-      d->q_heads % d->kv_heads || d->head_dim < 1)
+      d->q_heads % d->kv_heads || d->head_dim < 1 || d->kv_tokens > INT_MAX - 1024)
     return DCNV2_ERR_INVALID_ARG;
   if (d->head_dim % 8 || d->head_dim > 128) return DCNV2_ERR_UNSUPPORTED;
   if (!(d->scale > 0.f && std::isfinite(d->scale))) return DCNV2_ERR_INVALID_ARG;

@@ -216,10 +216,29 @@ def attention_inputs(b, L, s, h, g, d, dtype, seed, spread=1.0):
     return q, k, v
 
 
+def attention_desc(q, k, v, out=None, scale=None):
+    B, L, H, D = q.shape
+    d = capi.AttentionDesc(B, L, k.shape[1], H, k.shape[2], D,
+                           int(capi.DType.BF16 if q.dtype == BF16 else capi.DType.HALF),
+                           scale or D ** -0.5)
+    for field, t in ((d.q_stride, q), (d.k_stride, k), (d.v_stride, v),
+                     (d.out_stride, q if out is None else out)):
+        field[:] = t.stride()[:3]
+    return d
+
+
 def run_attention(q, k, v, lens=None, mask=None, **kw):
+    """(out, lse) on the GPU, its error words read clear afterwards."""
     mv = lambda x: None if x is None else x.to(DEV)  # noqa: E731
-    return dcnv2_cross_attention(mv(q), mv(k), mv(v), kv_lens=mv(lens), key_mask=mv(mask),
-                                 return_lse=True, **kw)
+    q, k, v = mv(q), mv(k), mv(v)
+    desc = attention_desc(q.contiguous(), k, v)
+    ws = torch.full((max(1, capi.attention_workspace_size(desc)),), 255, dtype=torch.uint8,
+                    device=DEV)
+    res = dcnv2_cross_attention(q, k, v, kv_lens=mv(lens), key_mask=mv(mask), return_lse=True,
+                                workspace=ws, **kw)
+    st = torch.cuda.current_stream().cuda_stream
+    assert capi.cross_attention_error(desc, ws.data_ptr(), st) == 0
+    return res
 
 
 @pytest.mark.parametrize("dtype", [FP16, BF16])
@@ -238,6 +257,12 @@ def run_attention(q, k, v, lens=None, mask=None, **kw):
     (1, 1000, 700, 3, 3, 96),
     (2, 256, 384, 2, 1, 16),
     (1, 513, 130, 2, 2, 104),
+    (1, 2, 300, 256, 1, 64),       # a group of more rows than a tile, cut in two
+    (1, 3, 200, 131, 1, 64),       # a prime group of more than 128 heads
+    (1, 40, 260, 7, 1, 128),       # 18 tokens of 7 heads in a tile
+    (21, 300, 200, 4, 4, 64),      # more items than SMs: no split, several items per CTA
+    (20, 290, 150, 4, 4, 128),
+    (90, 20, 140, 2, 2, 32),       # one tile of rows, more items than SMs
 ])
 def test_attention_matches_formula(dtype, b, L, s, h, g, d):
     q, k, v = attention_inputs(b, L, s, h, g, d, dtype, b + L + s)
@@ -272,6 +297,23 @@ def test_attention_lengths_and_masks(dtype, L, h, g, d):
     check_attention(out, lse, q, k, v, lens, mask)
     out, lse = run_attention(q, k, v, lens, mask[2:3])  # one mask for all sequences
     check_attention(out, lse, q, k, v, lens, mask[2:3])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("by_mask", [False, True])
+def test_attention_runs_of_empty_sequences(d, by_mask):
+    """Several items per CTA, most sequences of the batch without a kept state, in long runs: by
+    their length or by their mask; the last and the first one too."""
+    b, L, s, h = 64, 260, 300, 2
+    q, k, v = attention_inputs(b, L, s, h, h, d, BF16, d)
+    lens = torch.zeros(b, dtype=torch.int32)
+    lens[[7, 8, 40, 50]] = torch.tensor([300, 1, 129, 128], dtype=torch.int32)
+    mask = torch.arange(s) < lens[:, None]
+    out, lse = run_attention(q, k, v, **({"mask": mask} if by_mask else {"lens": lens}))
+    some = [0, 7, 8, 39, 40, 41, 50, 63]
+    check_attention(out[some], lse[some], q[some], k[some], v[some], lens[some])
+    gone = (lens == 0).nonzero()[:, 0].to(DEV)
+    assert not bool(out[gone].any()) and bool((lse[gone] == -math.inf).all())
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, -65504.0])
@@ -335,6 +377,45 @@ def test_attention_strides_layouts_and_shared_states():
     assert torch.equal(dcnv2_cross_attention(qe, k, v), dcnv2_cross_attention(qe.contiguous(), k, v))
 
 
+@pytest.mark.parametrize("d", [40, 64, 72, 128])
+def test_attention_outputs_beside_others(d):
+    """Outputs as a view of a wider buffer, with more items than SMs (whole tiles of rows leave at
+    once): the places around them stay as they were."""
+    b, L, s, h = 30, 273, 90, 3
+    q, k, v = (x.to(DEV) for x in attention_inputs(b, L, s, h, h, d, FP16, d))
+    want = dcnv2_cross_attention(q, k, v)
+    wide = torch.full((b, L + 2, h + 1, 136), 7.0, dtype=FP16, device=DEV)
+    got = dcnv2_cross_attention(q, k, v, out=wide[:, 1:-1, 1:, :d])
+    assert torch.equal(got, want)
+    wide[:, 1:-1, 1:, :d] = 7
+    assert bool((wide == 7).all())
+    check_attention(want[:2], dcnv2_cross_attention(q, k, v, return_lse=True)[1][:2],
+                    q[:2].cpu(), k[:2].cpu(), v[:2].cpu())
+
+
+def test_attention_shared_query_and_two_streams_at_once():
+    """One query for all sequences (batch stride 0) on each kernel; two calls at once on two streams,
+    each with a workspace of its own, give the bits they give alone."""
+    for L in (1, 30, 200):
+        q, k, v = (x.to(DEV) for x in attention_inputs(3, L, 400, 4, 2, 64, BF16, L))
+        qe = q[:1].expand(3, L, 4, 64)
+        assert torch.equal(dcnv2_cross_attention(qe, k, v),
+                           dcnv2_cross_attention(qe.contiguous(), k, v))
+    a = [x.to(DEV) for x in attention_inputs(4, 900, 3000, 8, 8, 64, FP16, 1)]
+    b = [x.to(DEV) for x in attention_inputs(8, 1, 20000, 16, 2, 128, BF16, 2)]
+    want = dcnv2_cross_attention(*a), dcnv2_cross_attention(*b)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, (st, args) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(st):
+                got[i].append(dcnv2_cross_attention(*args))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_attention_large_offsets():
     """States behind 2^31 elements: a token stride of 2^23 elements over 300 tokens."""
     s, d, step = 300, 64, 2 ** 23
@@ -364,17 +445,14 @@ def test_attention_no_states_and_empty_batches():
 
 def test_attention_same_bits_every_time_and_error_word_clear():
     q, k, v = (x.to(DEV) for x in attention_inputs(2, 1, 9000, 8, 2, 128, BF16, 11))
-    desc = capi.AttentionDesc(2, 1, 9000, 8, 2, 128, int(capi.DType.BF16), 128 ** -0.5)
-    for field, t in ((desc.q_stride, q), (desc.k_stride, k), (desc.v_stride, v)):
-        field[:] = t.stride()[:3]
-    desc.out_stride[:] = q.stride()[:3]
-    n = capi.attention_workspace_size(desc)
-    ws = torch.full((n,), 255, dtype=torch.uint8, device=DEV)  # needs no setting up
-    first = dcnv2_cross_attention(q, k, v, workspace=ws)
+    first = dcnv2_cross_attention(q, k, v)
     for _ in range(20):
-        assert torch.equal(dcnv2_cross_attention(q, k, v, workspace=ws), first)
-    st = torch.cuda.current_stream().cuda_stream
-    assert capi.cross_attention_error(desc, ws.data_ptr(), st) == 0
+        assert torch.equal(dcnv2_cross_attention(q, k, v), first)
+    q, k, v = (x.to(DEV) for x in attention_inputs(2, 60, 9000, 8, 2, 128, BF16, 12))
+    first, lse = run_attention(q, k, v)  # (a workspace that holds anything, read clear)
+    for _ in range(20):
+        again = run_attention(q, k, v)
+        assert torch.equal(again[0], first) and torch.equal(again[1], lse)
 
 
 def test_refusals_on_the_device():

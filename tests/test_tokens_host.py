@@ -120,6 +120,10 @@ def attention(d, q=P, k=P, v=P, lens=None, mask=None, out=P, lse=P, ws=P, ws_byt
     (dict(strides={"v": (38400, 128, 68)}), Status.ERR_UNSUPPORTED),
     (dict(strides={"k": (-8, 128, 64)}), Status.ERR_INVALID_ARG),
     (dict(strides={"out": (0, 512, 64)}), Status.ERR_INVALID_ARG),
+    (dict(strides={"q": (2560, 0, 64)}), Status.ERR_UNSUPPORTED),   # shared along tokens, heads
+    (dict(strides={"q": (2560, 512, 0)}), Status.ERR_UNSUPPORTED),
+    (dict(strides={"k": (38400, 0, 64)}), Status.ERR_UNSUPPORTED),
+    (dict(kv_tokens=2 ** 31 - 1), Status.ERR_INVALID_ARG),
     (dict(strides={"mask": -300}), Status.ERR_INVALID_ARG),
     (dict(batch=1 << 20, q_tokens=1 << 20), Status.ERR_INVALID_ARG),
 ])
@@ -143,6 +147,8 @@ def test_attention_pointer_refusals_and_no_ops():
     assert attention(d, ws=None) == Status.ERR_WORKSPACE
     assert attention(d, ws=P + 2) == Status.ERR_WORKSPACE
     assert attention(d, ws_bytes=0) == Status.ERR_WORKSPACE
+    few = attention_desc(q_tokens=1)  # no workspace for up to 16 rows per kv head
+    assert lib.dcnv2_cross_attention_workspace_size(ctypes.byref(few)) == 0
     assert attention(attention_desc(batch=0)) == Status.OK
     assert attention(attention_desc(q_tokens=0), q=None, out=None) == Status.OK
     if not torch.cuda.is_available():
@@ -155,6 +161,11 @@ def test_attention_pointer_refusals_and_no_ops():
     code = ctypes.c_int32(0)
     assert lib.dcnv2_cross_attention_read_error(ctypes.byref(d), None, None,
                                                 ctypes.byref(code)) == bad
+    assert lib.dcnv2_cross_attention_read_error(ctypes.byref(few), None, None, None) == bad
+    code.value = 5
+    assert lib.dcnv2_cross_attention_read_error(ctypes.byref(few), None, None,
+                                                ctypes.byref(code)) == Status.OK
+    assert code.value == 0
 
 
 def test_rotary_tables():
