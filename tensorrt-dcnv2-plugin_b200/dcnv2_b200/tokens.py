@@ -21,7 +21,7 @@ import math
 from typing import Sequence
 
 from . import capi
-from .capi import AttentionDesc, DCNv2Error, DType, Norm, RotaryDesc, Status, lib
+from .capi import AttentionDesc, DCNv2Error, DType, Norm, RotaryDesc, lib
 
 
 @functools.lru_cache(maxsize=None)
@@ -58,13 +58,6 @@ def _current(index):
     if torch.cuda.current_device() != index:
         return None
     return torch._C._cuda_getCurrentRawStream(index)
-
-
-_NOTHING = contextlib.nullcontext()
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _check(what, name, meta, dtype, index, ndim):
@@ -199,7 +192,8 @@ def _rotary_plan(q, k, q_out, k_out, positions, freqs, q_weight, k_weight, pair_
             field[:] = t[1][:3]
             out_field[:] = o[1][:3] if o is not None else _packed(t[0])
     d.pos_batch_stride = pos_sb
-    return d, index, 0 in (B, T, D) or not (d.q_heads or d.k_heads)
+    # (a reference to d keeps it)
+    return ctypes.byref(d), index, 0 in (B, T, D) or not (d.q_heads or d.k_heads)
 
 
 def dcnv2_qk_norm_rotary(q, k=None, positions=None, freqs=None, pair_axis=b"", q_weight=None,
@@ -221,17 +215,30 @@ def dcnv2_qk_norm_rotary(q, k=None, positions=None, freqs=None, pair_axis=b"", q
         _meta(q), _meta(k), _meta(q_out), _meta(k_out), _meta(positions), _meta(freqs),
         _meta(q_weight), _meta(k_weight), bytes(pair_axis), norm, float(eps), bool(interleaved))
     st = _current(index) if stream is None else None
-    with _NOTHING if st is not None else _on(index, stream) as other:
-        if q is not None and q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        if k is not None and k_out is None:
-            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-        if nothing:
-            return q_out, k_out
-        rc = lib.dcnv2_qk_norm_rotary(
-            ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(positions), _ptr(freqs), _ptr(q_weight),
-            _ptr(k_weight), _ptr(q_out), _ptr(k_out), other if st is None else st)
-    if rc != Status.OK:
+    if st is None:
+        with _on(index, stream) as st:
+            return _rotary_launch(desc, nothing, q, k, positions, freqs, q_weight, k_weight, q_out,
+                                  k_out, st)
+    return _rotary_launch(desc, nothing, q, k, positions, freqs, q_weight, k_weight, q_out, k_out, st)
+
+
+def _rotary_launch(desc, nothing, q, k, positions, freqs, q_weight, k_weight, q_out, k_out, st):
+    import torch
+    if q is not None and q_out is None:
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is not None and k_out is None:
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if nothing:
+        return q_out, k_out
+    rc = lib.dcnv2_qk_norm_rotary(
+        desc, q if q is None else q.data_ptr(), k if k is None else k.data_ptr(),
+        positions if positions is None else positions.data_ptr(),
+        freqs if freqs is None else freqs.data_ptr(),
+        q_weight if q_weight is None else q_weight.data_ptr(),
+        k_weight if k_weight is None else k_weight.data_ptr(),
+        q_out if q_out is None else q_out.data_ptr(), k_out if k_out is None else k_out.data_ptr(),
+        st)
+    if rc:
         raise DCNv2Error(rc, "dcnv2_qk_norm_rotary")
     return q_out, k_out
 
@@ -276,7 +283,9 @@ def _attention_plan(q, k, v, out, kv_lens, key_mask, scale):
         field[:] = tuple(st if n > 1 else 0 for st, n in zip(strides, shape[:3]))
     d.mask_batch_stride = mask_sb
     nothing = 0 in (B, L, H, D)
-    return (d, 0 if nothing else capi.attention_workspace_size(d), index, (B, H, L), nothing)
+    # (a reference to d keeps it)
+    return (ctypes.byref(d), 0 if nothing else capi.attention_workspace_size(d), index, (B, H, L),
+            nothing)
 
 
 def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
@@ -302,19 +311,32 @@ def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
     if workspace is not None and workspace.get_device() != index:
         raise ValueError(f"dcnv2_cross_attention: workspace is not on cuda:{index}")
     st = _current(index) if stream is None else None
-    with _NOTHING if st is not None else _on(index, stream) as other:
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device) if return_lse else None
-        if nothing:
-            return (out, lse) if return_lse else out
-        if workspace is None or workspace.nbytes < ws_bytes:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes \
-                else None
-        rc = lib.dcnv2_cross_attention(
-            ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(kv_lens), _ptr(key_mask),
-            _ptr(out), _ptr(lse), _ptr(workspace), workspace.nbytes if workspace is not None else 0,
-            other if st is None else st)
-    if rc != Status.OK:
-        raise DCNv2Error(rc, "dcnv2_cross_attention")
+    if st is None:
+        with _on(index, stream) as st:
+            out, lse = _attention_launch(desc, ws_bytes, nothing, q, k, v, kv_lens, key_mask, out,
+                                         lse_shape if return_lse else None, workspace, st)
+    else:
+        out, lse = _attention_launch(desc, ws_bytes, nothing, q, k, v, kv_lens, key_mask, out,
+                                     lse_shape if return_lse else None, workspace, st)
     return (out, lse) if return_lse else out
+
+
+def _attention_launch(desc, ws_bytes, nothing, q, k, v, kv_lens, key_mask, out, lse_shape, workspace,
+                      st):
+    import torch
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty(lse_shape, dtype=torch.float32) if lse_shape is not None else None
+    if nothing:
+        return out, lse
+    if ws_bytes and (workspace is None or workspace.nbytes < ws_bytes):
+        workspace = q.new_empty((ws_bytes,), dtype=torch.uint8)
+    rc = lib.dcnv2_cross_attention(
+        desc, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+        kv_lens if kv_lens is None else kv_lens.data_ptr(),
+        key_mask if key_mask is None else key_mask.data_ptr(), out.data_ptr(),
+        lse if lse is None else lse.data_ptr(),
+        workspace if workspace is None else workspace.data_ptr(), ws_bytes, st)
+    if rc:
+        raise DCNv2Error(rc, "dcnv2_cross_attention")
+    return out, lse
