@@ -43,9 +43,7 @@
 
 namespace dcnv2 {
 
-constexpr int kAttnTile = 128;                 // states per tile, rows per MMA
-constexpr int kAttnThreads = 12 * 32;
-constexpr int kAttnProducerWarp = 8, kAttnMmaWarp = 9, kAttnFixWarp = 10;  // (11 only fills up)
+constexpr int kAttnTile = 128;                 // rows of a tile (MMA M, tensor-memory lanes)
 constexpr uint32_t kAttnBlockBytes = kAttnTile * 128;  // 128 rows of one 128-byte swizzle block
 constexpr int kAttnMaxSplit = 8;               // CTAs of a cluster (portable size)
 constexpr float kAttnLazy = 8.f;               // log2 of the growth that rescales
@@ -81,32 +79,41 @@ struct AttnArgs {
 // Shared-memory layout of an instance (bytes from a 1024-aligned base).
 template <int DP, bool PAIRED>
 struct AttnLayout {
+  // softmax warpgroups, and states per tile: S and O of all of them fill tensor memory
+  static constexpr int kWGs = !PAIRED && DP == 64 ? 4 : 2;
+  static constexpr int kN = 256 / kWGs;
+  static constexpr int kWords = kN / 32;                          // kept-state words of a tile
+  static constexpr int kThreads = (kWGs + 1) * 128;
+  static constexpr int kProducerWarp = kWGs * 4, kMmaWarp = kProducerWarp + 1,
+                       kFixWarp = kProducerWarp + 2;              // (the last one only fills up)
   static constexpr int kBlocks = DP / 64;                         // swizzle blocks of a row
-  static constexpr uint32_t kTileBytes = kBlocks * kAttnBlockBytes;
-  static constexpr int kQTiles = PAIRED ? 1 : 2;
-  static constexpr int kStages = DP == 128 ? (PAIRED ? 3 : 2) : (PAIRED ? 6 : 4);
+  static constexpr uint32_t kTileBytes = kBlocks * kAttnBlockBytes;  // of Q or O
+  static constexpr uint32_t kStateBlock = kN * 128;
+  static constexpr uint32_t kStateBytes = kBlocks * kStateBlock;  // of K or V
+  static constexpr int kQTiles = PAIRED ? 1 : kWGs;
+  static constexpr int kStages = DP == 128 ? (PAIRED ? 3 : 2) : 6;
   static constexpr int kInfos = kStages + 2;
   // O on its way out: beside Q, so that the next item's Q can come early, or, where shared memory
   // is short, over it
   static constexpr bool kOutBeside = !PAIRED && DP == 64;
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kK = kQTiles * kTileBytes;
-  static constexpr uint32_t kV = kK + kStages * kTileBytes;
-  static constexpr uint32_t kOut = kOutBeside ? kV + kStages * kTileBytes : kQ;
+  static constexpr uint32_t kV = kK + kStages * kStateBytes;
+  static constexpr uint32_t kOut = kOutBeside ? kV + kStages * kStateBytes : kQ;
   static constexpr uint32_t kInfo =                               // kInfos x 32 bytes
-      kV + kStages * kTileBytes + (kOutBeside ? 2 * kTileBytes : 0);
+      kV + kStages * kStateBytes + (kOutBeside ? kWGs * kTileBytes : 0);
   static constexpr uint32_t kBars = kInfo + kInfos * 32;
-  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 11;
+  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 5 * kWGs + 1;
   static constexpr uint32_t kDrain = kBars + (kNumBars - 1) * 8;  // the MMA issuer's own
   static constexpr uint32_t kFlags = kBars + kNumBars * 8;        // [kStages] of the K tiles
   static constexpr uint32_t kSlot = kFlags + kStages * 4;         // TMEM address, abort flag
   static constexpr uint32_t kBytes = kSlot + 16;
-  // at the end, over K and V: fp32 O of the two warpgroups; over Q: their (maximum, sum)
+  // at the end, over K, V and what follows: fp32 O of the warpgroups; over Q: their (maximum, sum)
   static constexpr uint32_t kPart = kK;
   static constexpr uint32_t kPartBytes = kAttnTile * DP * 4;
-  static_assert(2 * kPartBytes <= 2 * kStages * kTileBytes, "parts fit over K and V");
-  static_assert(2 * kAttnTile * 8 + (PAIRED ? kAttnTile : 2 * kAttnTile) *
-                                        (PAIRED ? 2 : 1) * kAttnMaxSplit * 4 <= kK,
+  static_assert(kPart + kWGs * kPartBytes <= kInfo, "parts fit over K, V and O");
+  static constexpr uint32_t kShare = kQ + kWGs * kAttnTile * 8;   // [row][part] factors, behind these
+  static_assert(kShare + kQTiles * kAttnTile * (PAIRED ? 2 : 1) * kAttnMaxSplit * 4 <= kK,
                 "statistics and shares fit over Q");
 };
 template <int DP, bool PAIRED>
@@ -129,14 +136,14 @@ constexpr uint32_t kInfoEmpty = 2;  // no tile: the item has no kept state
 constexpr uint32_t kTileEnd = 2, kTileSkip = 4;
 
 template <int DP, bool PAIRED, bool BF16>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     dcnv2_cross_attention_kernel(const __grid_constant__ AttnArgs args,
                                  const __grid_constant__ CUtensorMap tmap_q,
                                  const __grid_constant__ CUtensorMap tmap_k,
                                  const __grid_constant__ CUtensorMap tmap_v,
                                  const __grid_constant__ CUtensorMap tmap_o) {
   using LY = AttnLayout<DP, PAIRED>;
-  constexpr int NS = LY::kStages, NI = LY::kInfos;
+  constexpr int NS = LY::kStages, NI = LY::kInfos, WG = LY::kWGs, N = LY::kN, NW = LY::kWords;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -149,11 +156,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t v_empty = v_ready + 8 * NS;           // [NS] its products done
   const uint32_t info_full = v_empty + 8 * NS;         // [NI] words and flags of a tile
   const uint32_t info_empty = info_full + 8 * NI;      // [NI] read by everyone
-  const uint32_t s_full = info_empty + 8 * NI;         // [2] scores of warpgroup w
-  const uint32_t p_ready = s_full + 16;                // [2] its probabilities
-  const uint32_t q_full = p_ready + 16;                // [2] Q tile of warpgroup w
-  const uint32_t q_empty = q_full + 16;                // [2] its last scores done
-  const uint32_t o_full = q_empty + 16;                // [2] O of warpgroup w complete
+  const uint32_t s_full = info_empty + 8 * NI;         // [WG] scores of warpgroup w
+  const uint32_t p_ready = s_full + 8 * WG;            // [WG] its probabilities
+  const uint32_t q_full = p_ready + 8 * WG;            // [WG] Q tile of warpgroup w
+  const uint32_t q_empty = q_full + 8 * WG;            // [WG] its last scores done, O has left
+  const uint32_t o_full = q_empty + 8 * WG;            // [WG] O of warpgroup w complete
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + LY::kSlot);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   uint32_t* infos = reinterpret_cast<uint32_t*>(smem + LY::kInfo);  // words 0-3, flags
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   };
   auto item_at = [&](int item) {
     Item it;
-    it.tok0 = (item % args.row_tiles) * args.tile_tokens * (PAIRED ? 1 : 2);
+    it.tok0 = (item % args.row_tiles) * args.tile_tokens * LY::kQTiles;
     const int rest = item / args.row_tiles;
     it.g = rest % args.groups;
     it.b = rest / args.groups;
@@ -192,9 +199,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < NI; ++i) {
       ptx::mbar_init(info_full + 8 * i, 1);
-      ptx::mbar_init(info_empty + 8 * i, 9);  // softmax warps, V fixer
+      ptx::mbar_init(info_empty + 8 * i, WG * 4 + 1);  // softmax warps, V fixer
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < WG; ++i) {
       ptx::mbar_init(s_full + 8 * i, 1);
       ptx::mbar_init(p_ready + 8 * i, 4);
       ptx::mbar_init(q_full + 8 * i, 1);
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  if (warp == kAttnMmaWarp) {
+  if (warp == LY::kMmaWarp) {
     ptx::tmem_alloc(ptx::smem_addr(slot), 512);
     ptx::tmem_relinquish();
   }
@@ -216,30 +223,37 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   __syncthreads();
   ptx::tc_fence_after();
   const uint32_t tmem = *slot;
-  // tensor memory: scores of warpgroup w at 128 w (the probabilities over their first half), its O
-  // at 256 + DP w
+  // tensor memory: scores of warpgroup w at N w (the probabilities over their first half), its O at
+  // 256 + DP w
   const int w = warp >> 2;  // softmax warpgroup
   const float c = args.scale * kLog2e;
   // fp16 probabilities are scaled by 2^7 (at most 2^15): small ones keep their bits longer
   const float shift = BF16 ? 0.f : 7.f;
 
   // Reads entry n of the producer's ring: words of the tile and flags. False after an abort.
-  auto read_info = [&](int n, uint32_t (&word)[4], uint32_t& flags, int code) {
+  auto read_info = [&](int n, uint32_t (&word)[NW], uint32_t& flags, int code) {
     const bool ok = wait_bar<kSuspend>(info_full + 8 * (n % NI),
                                        static_cast<uint32_t>(n / NI) & 1u, wc, code);
     if (!__all_sync(0xffffffffu, ok)) return false;
     const uint4 f = ptx::ld_shared_v4(base + LY::kInfo + (n % NI) * 32);
-    word[0] = f.x; word[1] = f.y; word[2] = f.z; word[3] = f.w;
+    word[0] = f.x;
+    word[1] = f.y;
+    if constexpr (NW == 4) {
+      word[2] = f.z;
+      word[3] = f.w;
+    }
     flags = ptx::ld_shared_u32_volatile(base + LY::kInfo + (n % NI) * 32 + 16);
     __syncwarp();
     if (lane == 0) ptx::mbar_arrive(info_empty + 8 * (n % NI));
     return true;
   };
 
-  // 384 threads x 168 registers at launch cover 256 x 192 + 128 x 120
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-  if (warp == kAttnProducerWarp) {
+  // two softmax warpgroups: 384 threads x 168 registers at launch cover 256 x 192 + 128 x 120;
+  // four: 640 x 96 cover 512 x 104 + 128 x 64
+  if (warp >= LY::kProducerWarp) {
+  if constexpr (WG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if (warp == LY::kProducerWarp) {
     // ------------------------------------------------------------ producer
     int n = 0, i = 0;                    // ring entries, tiles
     uint32_t skipped = 0;                // items without a tile since the last one with tiles
@@ -249,38 +263,41 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const Item it = item_at(item);
       int len = args.S;
       if (args.kv_lens) len = max(0, min(len, __ldg(args.kv_lens + it.b)));
-      const int tiles = (len + kAttnTile - 1) / kAttnTile;
+      const int tiles = (len + N - 1) / N;
       const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / args.split);
       int t = static_cast<int>(static_cast<int64_t>(tiles) * rank / args.split);
       const uint8_t* mask = args.key_mask ? args.key_mask + it.b * args.mask_sb : nullptr;
-      uint8_t next[4];  // the lane's mask bytes of tile t
+      uint8_t next[NW];  // the lane's mask bytes of tile t
       auto fetch = [&](int tile) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int j = tile * kAttnTile + x * 32 + lane;
+        for (int x = 0; x < NW; ++x) {
+          const int j = tile * N + x * 32 + lane;
           next[x] = tile < t1 && j < len ? __ldg(mask + j) : 0;
         }
       };
       // the next tile with a kept state from t on (t moves behind it), or -1
-      auto find = [&](uint32_t (&word)[4]) {
+      auto find = [&](uint32_t (&word)[NW]) {
         for (; t < t1; ++t) {
           if (!mask) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int left = len - t * kAttnTile - x * 32;
+            for (int x = 0; x < NW; ++x) {
+              const int left = len - t * N - x * 32;
               word[x] = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
             }
             return t++;
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) word[x] = __ballot_sync(0xffffffffu, next[x] != 0);
+          for (int x = 0; x < NW; ++x) word[x] = __ballot_sync(0xffffffffu, next[x] != 0);
           fetch(t + 1);
-          if ((word[0] | word[1] | word[2] | word[3]) != 0) return t++;
+          uint32_t some = 0;
+#pragma unroll
+          for (int x = 0; x < NW; ++x) some |= word[x];
+          if (some) return t++;
         }
         return -1;
       };
       if (mask) fetch(t);
-      uint32_t word[4] = {0, 0, 0, 0}, word_next[4];
+      uint32_t word[NW] = {}, word_next[NW];
       int tile = find(word);
       uint32_t flags = tile < 0 ? (kInfoEmpty | kInfoLast) : 0;
       do {
@@ -293,7 +310,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                                   wc, DCNV2_DEVERR_TIMEOUT_PRODUCER);
           if (ok) {
             uint32_t* f = infos + at * 8;
-            f[0] = word[0]; f[1] = word[1]; f[2] = word[2]; f[3] = word[3];
+#pragma unroll
+            for (int x = 0; x < NW; ++x) f[x] = word[x];
             f[4] = flags;
             ptx::mbar_arrive(info_full + 8 * at);
             if (tile >= 0)
@@ -302,19 +320,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           }
           if (ok && tile >= 0) {
             tile_flags[s] = (flags & kInfoLast) + skipped * kTileSkip;
-            ptx::mbar_arrive_expect_tx(k_full + 8 * s, LY::kTileBytes);
+            ptx::mbar_arrive_expect_tx(k_full + 8 * s, LY::kStateBytes);
             for (int x = 0; x < LY::kBlocks; ++x)
-              ptx::tma_load_4d(base + LY::kK + s * LY::kTileBytes + x * kAttnBlockBytes, &tmap_k,
-                               x * 64, tile * kAttnTile, (it.g / args.kv_parts) * args.k_head,
+              ptx::tma_load_4d(base + LY::kK + s * LY::kStateBytes + x * LY::kStateBlock, &tmap_k,
+                               x * 64, tile * N, (it.g / args.kv_parts) * args.k_head,
                                it.b * args.k_batch,
                                k_full + 8 * s);
             k_ahead = true;
             ok = wait_bar<kSuspend>(v_empty + 8 * s, ph ^ 1u, wc, DCNV2_DEVERR_TIMEOUT_PRODUCER);
             if (ok) {
-              ptx::mbar_arrive_expect_tx(v_full + 8 * s, LY::kTileBytes);
+              ptx::mbar_arrive_expect_tx(v_full + 8 * s, LY::kStateBytes);
               for (int x = 0; x < LY::kBlocks; ++x)
-                ptx::tma_load_4d(base + LY::kV + s * LY::kTileBytes + x * kAttnBlockBytes,
-                                 &tmap_v, x * 64, tile * kAttnTile,
+                ptx::tma_load_4d(base + LY::kV + s * LY::kStateBytes + x * LY::kStateBlock,
+                                 &tmap_v, x * 64, tile * N,
                                  (it.g / args.kv_parts) * args.v_head, it.b * args.v_batch, v_full + 8 * s);
               k_ahead = false;
             }
@@ -328,7 +346,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tile = tile_next;
         flags = 0;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) word[x] = word_next[x];
+        for (int x = 0; x < NW; ++x) word[x] = word_next[x];
       } while (tile >= 0);
     }
     if (lane == 0) {
@@ -349,7 +367,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         drain_bar(v_full + 8 * (x % NS), static_cast<uint32_t>(x / NS) & 1u, wc);
       if (k_ahead) drain_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc);
     }
-  } else if (warp == kAttnMmaWarp) {
+  } else if (warp == LY::kMmaWarp) {
     // ------------------------------------------------------------ MMA issuer
     // The warp runs this code as a whole, one elected lane issues. As little as possible stands between
     // the arrival of probabilities and the MMAs they release: what the next tile is, and that its K is
@@ -358,19 +376,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     // each other (16 heads of 128, 4096 x 16384: 656 us, this 500 us).
     constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
     const bool leader = ptx::elect_one();
-    const uint32_t id_s = ptx::make_idesc(1, fmt, kAttnTile);
+    const uint32_t id_s = ptx::make_idesc(1, fmt, N);
     const uint32_t id_o =
         ptx::make_idesc(1, fmt, static_cast<uint32_t>((args.D + 15) / 16 * 16)) | ptx::kIdescBMn;
     const int d_steps = (args.D + 15) / 16;
     const uint64_t q_desc = ptx::sw128_kmajor_desc(base + LY::kQ);
     const uint64_t k_desc = ptx::sw128_kmajor_desc(base + LY::kK);
-    const uint64_t v_desc = ptx::sw128_mnmajor_desc(base + LY::kV, kAttnBlockBytes);
+    const uint64_t v_desc = ptx::sw128_mnmajor_desc(base + LY::kV, LY::kStateBlock);
     const uint32_t q_lo = static_cast<uint32_t>(q_desc), k_lo = static_cast<uint32_t>(k_desc);
     const uint32_t v_lo = static_cast<uint32_t>(v_desc);
     const uint32_t kd_hi = static_cast<uint32_t>(k_desc >> 32);
     const uint32_t v_hi = static_cast<uint32_t>(v_desc >> 32);
     bool ok = true;
-    uint32_t q_loads[2] = {0, 0}, p_turn[2] = {0, 0};
+    uint32_t q_loads[WG] = {}, p_turn[WG] = {};
     auto wait = [&](uint32_t bar, uint32_t parity) {
       const bool got = wait_bar(bar, parity & 1u, wc, DCNV2_DEVERR_TIMEOUT_MMA);
       return ok = __all_sync(0xffffffffu, ok && got);
@@ -393,7 +411,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     // tile i: whether there is one (its K is there then), and of which item
     int item = item0;
     Item it = item_at(item0);
-    bool begun = false, fresh = true, last = true, both = false;
+    bool begun = false, fresh = true, last = true;
+    int active = 0;  // warpgroups with rows of the item
     auto next_tile = [&](int i) {
       if (!wait(k_full + 8 * (i % NS), i / NS)) return false;
       const uint32_t flags = ptx::ld_shared_u32_volatile(base + LY::kFlags + (i % NS) * 4);
@@ -404,22 +423,22 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         item += item_step * static_cast<int>(flags / kTileSkip + (begun ? 1 : 0));
         it = item_at(item);
         begun = true;
-        both = rows_of(it, 1) > 0;
+        for (active = 0; active < LY::kQTiles && rows_of(it, active) > 0;) ++active;
       }
       return true;
     };
     auto scores = [&](int i, int wg) {  // S of warpgroup wg from K tile i
       const uint32_t q = q_lo + (PAIRED ? 0 : wg) * (LY::kTileBytes >> 4);
-      const uint32_t k = k_lo + (i % NS) * (LY::kTileBytes >> 4);
-      const uint32_t d = tmem + kAttnTile * wg;
+      const uint32_t k = k_lo + (i % NS) * (LY::kStateBytes >> 4);
+      const uint32_t d = tmem + N * wg;
       ptx::tc_fence_after();
       if (leader) {
         ptx::mma_f16_run<false>(d, q, kd_hi, k, kd_hi, id_s);
 #pragma unroll
         for (int x = 1; x < DP / 16; ++x) {
-          constexpr uint32_t kBlock = kAttnBlockBytes >> 4;
-          const uint32_t off = (x >> 2) * kBlock + (x & 3) * 2;
-          if (x < d_steps) ptx::mma_f16_run<true>(d, q + off, kd_hi, k + off, kd_hi, id_s);
+          const uint32_t q_off = (x >> 2) * (kAttnBlockBytes >> 4) + (x & 3) * 2;
+          const uint32_t k_off = (x >> 2) * (LY::kStateBlock >> 4) + (x & 3) * 2;
+          if (x < d_steps) ptx::mma_f16_run<true>(d, q + q_off, kd_hi, k + k_off, kd_hi, id_s);
         }
         ptx::tc_commit(s_full + 8 * wg);
       }
@@ -428,11 +447,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     auto product = [&](int i, int wg, bool first) {  // O of warpgroup wg += P V tile i
       if (!wait(p_ready + 8 * wg, p_turn[wg]++)) return false;
       ptx::tc_fence_after();
-      const uint32_t v = v_lo + (i % NS) * (LY::kTileBytes >> 4);
-      const uint32_t d = tmem + 2 * kAttnTile + DP * wg, p = tmem + kAttnTile * wg;
+      const uint32_t v = v_lo + (i % NS) * (LY::kStateBytes >> 4);
+      const uint32_t d = tmem + 256 + DP * wg, p = tmem + N * wg;
       if (leader) {
 #pragma unroll
-        for (int x = 0; x < kAttnTile / 16; ++x)
+        for (int x = 0; x < N / 16; ++x)
           ptx::mma_f16_ta_run(d, p + 8 * x, v + x * (2048 >> 4), v_hi, id_o,
                               x > 0 ? 1u : first ? 0u : 1u);
       }
@@ -470,11 +489,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     } else {
       bool have = next_tile(0);
       if (have)
-        for (int wg = 0; wg <= both; ++wg) load_q(it, wg);
+        for (int wg = 0; wg < active; ++wg) load_q(it, wg);
       int i = 0;
       while (have && ok) {  // an item begins: its Q is on its way
-        const bool cur_both = both;
-        for (int wg = 0; wg <= cur_both; ++wg)
+        const int cur_active = active;
+        for (int wg = 0; wg < cur_active; ++wg)
           if (wait(q_full + 8 * wg, q_loads[wg] - 1)) scores(i, wg);
         commit(k_empty + 8 * (i % NS));
         bool first = true, ends = false;
@@ -485,7 +504,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           // items in between are read by the softmax only when this item's O is complete.
           if (!ends) next_tile(i);
           if (!wait(v_ready + 8 * at, cur / NS)) break;
-          for (int wg = 0; wg <= cur_both; ++wg) {
+          for (int wg = 0; wg < cur_active; ++wg) {
             if (!product(cur, wg, first)) break;
             if (ends) commit(o_full + 8 * wg);
             else scores(i, wg);
@@ -499,7 +518,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         have = next_tile(i);
         // the next item's Q: this one's scores are done, and where Q is O's way out, O has left it
         if (have)
-          for (int wg = 0; wg <= both; ++wg) {
+          for (int wg = 0; wg < active; ++wg) {
             if (!LY::kOutBeside && q_loads[wg] && !wait(q_empty + 8 * wg, q_loads[wg] - 1)) break;
             load_q(it, wg);
           }
@@ -509,16 +528,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     __syncwarp();
     commit(base + LY::kDrain);
     drain_bar(base + LY::kDrain, 0, wc);
-    for (int wg = 0; wg < 2; ++wg)
+    for (int wg = 0; wg < WG; ++wg)
       if (q_loads[wg]) drain_bar(q_full + 8 * wg, (q_loads[wg] - 1) & 1u, wc);
-  } else if (warp == kAttnFixWarp) {
+  } else if (warp == LY::kFixWarp) {
     // ------------------------------------------------------------ V rows of unkept states
     int n = 0, i = 0;
     bool ok = true;
     for (int item = item0; item < args.items && ok; item += item_step) {
       uint32_t flags = 0;
       while (ok && !(flags & kInfoLast)) {
-        uint32_t word[4];
+        uint32_t word[NW];
         ok = read_info(n, word, flags, DCNV2_DEVERR_TIMEOUT_PRODUCER);
         if (!ok) break;
         ++n;
@@ -528,14 +547,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
                                 DCNV2_DEVERR_TIMEOUT_PRODUCER);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if ((word[0] & word[1] & word[2] & word[3]) != 0xffffffffu) {
+        uint32_t whole = 0xffffffffu;
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < NW; ++x) whole &= word[x];
+        if (whole != 0xffffffffu) {
+#pragma unroll
+          for (int x = 0; x < NW; ++x)
             if (!((word[x] >> lane) & 1u)) {
-              const uint32_t row = base + LY::kV + s * LY::kTileBytes + (x * 32 + lane) * 128;
+              const uint32_t row = base + LY::kV + s * LY::kStateBytes + (x * 32 + lane) * 128;
               for (int y = 0; y < LY::kBlocks; ++y)
                 for (int z = 0; z < 8; ++z)
-                  ptx::st_shared_v4(row + y * kAttnBlockBytes + z * 16, make_uint4(0, 0, 0, 0));
+                  ptx::st_shared_v4(row + y * LY::kStateBlock + z * 16, make_uint4(0, 0, 0, 0));
             }
           ptx::fence_proxy_async_smem();
         }
@@ -551,11 +573,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     ptx::cluster_sync();
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (WG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ------------------------------------------------------------ softmax
     const int rl = (warp & 3) * 32 + lane;  // row of the tile = tensor-memory lane
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
-    const uint32_t t_s = tmem + lanes + kAttnTile * w, t_o = tmem + lanes + 2 * kAttnTile + DP * w;
+    const uint32_t t_s = tmem + lanes + N * w, t_o = tmem + lanes + 256 + DP * w;
     int n = 0, tile = 0;         // ring entries read; tiles of the item
     uint32_t s_turn = 0, o_turn = 0;
     bool ok = true;
@@ -568,7 +591,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       bool first = true, any = false;
       uint32_t flags = 0;
       for (tile = 0; !(flags & kInfoLast); ++tile) {
-        uint32_t word[4];
+        uint32_t word[NW];
         ok = read_info(n, word, flags, DCNV2_DEVERR_TIMEOUT_SAMPLER);
         if (!ok) break;
         ++n;
@@ -583,31 +606,31 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           if (lane == 0) ptx::mbar_arrive(p_ready + 8 * w);
           continue;
         }
-        uint32_t sc[4][32];
+        uint32_t sc[NW][32];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) ptx::tmem_ld_32x32b_x32(t_s + 32 * x, sc[x]);
+        for (int x = 0; x < NW; ++x) ptx::tmem_ld_32x32b_x32(t_s + 32 * x, sc[x]);
         ptx::tmem_wait_ld();
 #pragma unroll
-        for (int x = 0; x < 4; ++x) ptx::tmem_ld_use(sc[x]);
+        for (int x = 0; x < NW; ++x) ptx::tmem_ld_use(sc[x]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < NW; ++x)
           if (word[x] != 0xffffffffu) {
 #pragma unroll
             for (int y = 0; y < 32; ++y)
               if (!((word[x] >> y) & 1u)) sc[x][y] = 0xff800000u;  // -inf
           }
-        float top[8];
+        float top[2 * NW];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
+        for (int x = 0; x < 2 * NW; ++x) {
           const uint32_t* q = &sc[x >> 1][(x & 1) * 16];
           top[x] = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 #pragma unroll
           for (int y = 2; y < 16; y += 2)
             top[x] = ptx::max3(top[x], __uint_as_float(q[y]), __uint_as_float(q[y + 1]));
         }
-        top[0] = ptx::max3(top[0], top[1], top[2]);
-        top[3] = ptx::max3(top[3], top[4], top[5]);
-        top[0] = fmaxf(ptx::max3(top[0], top[3], top[6]), top[7]);
+#pragma unroll
+        for (int x = 2 * NW - 1; x > 1; x -= 2) top[0] = ptx::max3(top[0], top[x], top[x - 1]);
+        top[0] = fmaxf(top[0], top[1]);
         const float m = fmaxf(m_ref, top[0]);
         // (-inf) - (-inf) is NaN, which is not greater
         if (__any_sync(0xffffffffu, (m - m_ref) * c > kAttnLazy)) {
@@ -631,7 +654,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const float2 c2 = make_float2(c, c), n2 = make_float2(neg, neg);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < NW; ++x) {
           uint32_t pk[16];
 #pragma unroll
           for (int y = 0; y < 16; ++y) {
@@ -655,9 +678,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         bool done = ok && wait_bar<kSuspend>(o_full + 8 * w, o_turn & 1u, wc,
                                              DCNV2_DEVERR_TIMEOUT_EPILOGUE);
         if (PAIRED || args.split > 1)
-          done = done && (rows_of(item_at(item), w ^ 1) == 0 ||
-                          wait_bar<kSuspend>(o_full + 8 * (w ^ 1), o_turn & 1u, wc,
-                                             DCNV2_DEVERR_TIMEOUT_EPILOGUE));
+          for (int x = 0; x < WG; ++x)
+            done = done && (rows_of(item_at(item), x) == 0 ||
+                            wait_bar<kSuspend>(o_full + 8 * x, o_turn & 1u, wc,
+                                               DCNV2_DEVERR_TIMEOUT_EPILOGUE));
         ++o_turn;
         if (!__all_sync(0xffffffffu, done)) {
           l = NAN;  // shows in the result, beside the error word
@@ -753,15 +777,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         constexpr int MP = PAIRED ? 2 * kAttnMaxSplit : kAttnMaxSplit;
         const Item it = item_at(item0);
         const int parts = PAIRED ? 2 * args.split : args.split;
-        const int rows0 = rows_of(it, 0), n_rows = rows0 + (PAIRED ? 0 : rows_of(it, 1));
+        const int tile_rows = args.tile_tokens * args.heads;
+        int n_rows = 0;
+        for (int x = 0; x < LY::kQTiles; ++x) n_rows += rows_of(it, x);
         const int block = (n_rows + args.split - 1) / args.split;
         const int r0 = rank * block, r1 = min(n_rows, r0 + block);
         auto cta = [&](int y) { return PAIRED ? y >> 1 : y; };
-        auto wg = [&](int y, int r) { return PAIRED ? y & 1 : r < rows0 ? 0 : 1; };
-        auto tile_row = [&](int r) { return r < rows0 ? r : r - rows0; };
+        auto wg = [&](int y, int r) { return PAIRED ? y & 1 : r / tile_rows; };
+        auto tile_row = [&](int r) { return PAIRED ? r : r % tile_rows; };
+        auto token = [&](int r) { return it.tok0 + r / args.heads; };
         // behind the statistics that the other CTAs read: [row of the block][part] factors
-        float* share = reinterpret_cast<float*>(smem + LY::kQ + 2 * kAttnTile * 8);
-        for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += 256) {
+        float* share = reinterpret_cast<float*>(smem + LY::kShare);
+        for (int r = r0 + static_cast<int>(threadIdx.x); r < r1; r += WG * 128) {
           float2 ml[MP];
           float top = -INFINITY, total = 0.f;
 #pragma unroll
@@ -783,16 +810,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
           for (int y = 0; y < MP; ++y)
             if (y < parts) share[(r - r0) * MP + y] = ml[y].x * inv;
           if (args.lse) {
-            const int tr = tile_row(r);
-            const int tok = it.tok0 + (r < rows0 ? 0 : args.tile_tokens) + tr / args.heads;
-            const int h = it.g * args.heads + tr % args.heads;
-            args.lse[(static_cast<int64_t>(it.b) * args.H + h) * args.L + tok] =
+            const int h = it.g * args.heads + r % args.heads;
+            args.lse[(static_cast<int64_t>(it.b) * args.H + h) * args.L + token(r)] =
                 total == 0.f ? -INFINITY : kLn2 * (top * c - shift + log2f(total));
           }
         }
-        ptx::named_barrier(1, 256);
+        ptx::named_barrier(1, WG * 128);
         const int quads = args.D / 4;
-        for (int x = threadIdx.x; x < (r1 - r0) * quads; x += 256) {
+        for (int x = threadIdx.x; x < (r1 - r0) * quads; x += WG * 128) {
           const int rb = x / quads, r = r0 + rb, ch = x - rb * quads, tr = tile_row(r);
           float4 o[MP];
 #pragma unroll
@@ -808,10 +833,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
               acc.x = fmaf(o[y].x, f, acc.x); acc.y = fmaf(o[y].y, f, acc.y);
               acc.z = fmaf(o[y].z, f, acc.z); acc.w = fmaf(o[y].w, f, acc.w);
             }
-          const int tok = it.tok0 + (r < rows0 ? 0 : args.tile_tokens) + tr / args.heads;
-          const int h = it.g * args.heads + tr % args.heads;
+          const int h = it.g * args.heads + r % args.heads;
           *reinterpret_cast<uint2*>(static_cast<uint16_t*>(args.out) + it.b * args.out_sb +
-                                    tok * args.out_st + h * args.out_sh + ch * 4) =
+                                    token(r) * args.out_st + h * args.out_sh + ch * 4) =
               make_uint2(ptx::pack16<BF16>(acc.x, acc.y), ptx::pack16<BF16>(acc.z, acc.w));
         }
       }
@@ -819,7 +843,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   }
   __syncthreads();
-  if (warp == kAttnMmaWarp) {
+  if (warp == LY::kMmaWarp) {
     __syncwarp();
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);

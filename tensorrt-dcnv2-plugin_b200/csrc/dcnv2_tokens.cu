@@ -164,6 +164,7 @@ struct AttnPlan {
   bool step = false;       // few rows: dcnv2_attention_step_kernel
   bool paired = false;     // one tile of rows, the warpgroups alternate over the states
   bool wide = false;       // heads of more than 64 elements
+  int wgs = 2;             // softmax warpgroups
   int heads = 1, kv_parts = 1, tile_tokens = 1;  // rows of a tile (AttnArgs)
   int row_tiles = 0, items = 0, split = 1;
   unsigned grid = 0;
@@ -229,7 +230,9 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   p->kv_parts = group / p->heads;
   p->tile_tokens = kAttnTile / p->heads;
   p->paired = d->q_tokens <= p->tile_tokens;
-  p->row_tiles = static_cast<int>(cdiv(d->q_tokens, p->tile_tokens * (p->paired ? 1 : 2)));
+  p->wgs = !p->paired && !p->wide ? AttnLayout<64, false>::kWGs : AttnLayout<128, false>::kWGs;
+  p->row_tiles =
+      static_cast<int>(cdiv(d->q_tokens, int64_t(p->tile_tokens) * (p->paired ? 1 : p->wgs)));
   const int64_t groups = int64_t(d->kv_heads) * p->kv_parts;
   if (groups > INT_MAX || int64_t(d->batch) * groups > INT_MAX) return DCNV2_ERR_INVALID_ARG;
   const int64_t ctas = int64_t(d->batch) * groups * p->row_tiles;
@@ -261,11 +264,11 @@ bool encode_map(CUtensorMap* m, const void* p, int rank, const cuuint64_t* dims,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x 128 tokens in the
-// 128-byte swizzle. Axes that no step is taken along, or that share their states, have extent 1.
+// Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x the 256 / wgs tokens
+// of a tile in the 128-byte swizzle. Axes that no step is taken along, or that share their states, have extent 1.
 // What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
 bool states_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
-                const dcnv2_attention_desc& d, int* batch_step, int* head_step) {
+                const dcnv2_attention_desc& d, int wgs, int* batch_step, int* head_step) {
   const bool heads = d.kv_heads > 1 && stride[2] > 0, batch = d.batch > 1 && stride[0] > 0;
   *head_step = heads;
   *batch_step = batch;
@@ -277,7 +280,7 @@ bool states_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
   const cuuint64_t strides[3] = {d.kv_tokens > 1 ? static_cast<cuuint64_t>(stride[1]) * 2 : row,
                                  heads ? static_cast<cuuint64_t>(stride[2]) * 2 : row,
                                  batch ? static_cast<cuuint64_t>(stride[0]) * 2 : row};
-  const cuuint32_t box[4] = {64, kAttnTile, 1, 1};
+  const cuuint32_t box[4] = {64, 256u / static_cast<cuuint32_t>(wgs), 1, 1};
   return encode_map(m, p, 4, dims, strides, box);
 }
 
@@ -323,7 +326,7 @@ dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPl
   }
   cudaLaunchAttribute at[2];
   const cudaLaunchConfig_t cfg =
-      launch_config(p.grid, kAttnThreads, smem, st, at, static_cast<unsigned>(p.split));
+      launch_config(p.grid, AttnLayout<DP, PAIRED>::kThreads, smem, st, at, static_cast<unsigned>(p.split));
   return launched(cudaLaunchKernelEx(&cfg, kernel, a, m.q, m.k, m.v, m.o));
 }
 
@@ -525,8 +528,8 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
     return DCNV2_ERR_UNSUPPORTED;  // strides of 2^40 bytes and more
   if (d.kv_tokens == 0) {  // nothing is loaded
     m.k = m.v = m.q;
-  } else if (!states_map(&m.k, k, d.k_stride, d, &a.k_batch, &a.k_head) ||
-             !states_map(&m.v, v, d.v_stride, d, &a.v_batch, &a.v_head)) {
+  } else if (!states_map(&m.k, k, d.k_stride, d, p.wgs, &a.k_batch, &a.k_head) ||
+             !states_map(&m.v, v, d.v_stride, d, p.wgs, &a.v_batch, &a.v_head)) {
     return DCNV2_ERR_UNSUPPORTED;
   }
   return d.dtype == DCNV2_BF16 ? launch_attention<true>(a, m, p, dev, st)
