@@ -84,8 +84,9 @@ struct AttnLayout {
   static constexpr int kN = 256 / kWGs;
   static constexpr int kWords = kN / 32;                          // kept-state words of a tile
   static constexpr int kThreads = (kWGs + 1) * 128;
-  static constexpr int kProducerWarp = kWGs * 4, kMmaWarp = kProducerWarp + 1,
-                       kFixWarp = kProducerWarp + 2;              // (the last one only fills up)
+  static constexpr int kProducerWarp = kWGs * 4, kFixWarp = kProducerWarp + 1,
+                       kMmaWarp = kProducerWarp + 2;              // and the next, of kIssuers = 2
+  static constexpr int kIssuers = kWGs / 2;                       // each for two warpgroups
   static constexpr int kBlocks = DP / 64;                         // swizzle blocks of a row
   static constexpr uint32_t kTileBytes = kBlocks * kAttnBlockBytes;  // of Q or O
   static constexpr uint32_t kStateBlock = kN * 128;
@@ -103,8 +104,8 @@ struct AttnLayout {
   static constexpr uint32_t kInfo =                               // kInfos x 32 bytes
       kV + kStages * kStateBytes + (kOutBeside ? kWGs * kTileBytes : 0);
   static constexpr uint32_t kBars = kInfo + kInfos * 32;
-  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 5 * kWGs + 1;
-  static constexpr uint32_t kDrain = kBars + (kNumBars - 1) * 8;  // the MMA issuer's own
+  static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 5 * kWGs + kIssuers;
+  static constexpr uint32_t kDrain = kBars + (kNumBars - kIssuers) * 8;  // the MMA issuers' own
   static constexpr uint32_t kFlags = kBars + kNumBars * 8;        // [kStages] of the K tiles
   static constexpr uint32_t kSlot = kFlags + kStages * 4;         // TMEM address, abort flag
   static constexpr uint32_t kBytes = kSlot + 16;
@@ -192,10 +193,10 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       ptx::mbar_init(k_full + 8 * i, 1);
-      ptx::mbar_init(k_empty + 8 * i, 1);
+      ptx::mbar_init(k_empty + 8 * i, LY::kIssuers);
       ptx::mbar_init(v_full + 8 * i, 1);
       ptx::mbar_init(v_ready + 8 * i, 1);
-      ptx::mbar_init(v_empty + 8 * i, 1);
+      ptx::mbar_init(v_empty + 8 * i, LY::kIssuers);
     }
     for (int i = 0; i < NI; ++i) {
       ptx::mbar_init(info_full + 8 * i, 1);
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       ptx::mbar_init(q_empty + 8 * i, 1);
       ptx::mbar_init(o_full + 8 * i, 1);
     }
-    ptx::mbar_init(base + LY::kDrain, 1);
+    for (int i = 0; i < LY::kIssuers; ++i) ptx::mbar_init(base + LY::kDrain + 8 * i, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
@@ -367,13 +368,14 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         drain_bar(v_full + 8 * (x % NS), static_cast<uint32_t>(x / NS) & 1u, wc);
       if (k_ahead) drain_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc);
     }
-  } else if (warp == LY::kMmaWarp) {
+  } else if (warp >= LY::kMmaWarp && warp < LY::kMmaWarp + LY::kIssuers) {
     // ------------------------------------------------------------ MMA issuer
     // The warp runs this code as a whole, one elected lane issues. As little as possible stands between
     // the arrival of probabilities and the MMAs they release: what the next tile is, and that its K is
-    // there, is found out while the softmax works. One issuer serves the warpgroups in turn, which
-    // keeps them apart: two of their own let them fall into step, and MMAs and exponentials wait for
-    // each other (16 heads of 128, 4096 x 16384: 656 us, this 500 us).
+    // there, is found out while the softmax works. One issuer serves two warpgroups in turn, which
+    // keeps them apart: with one each they fall into step, and MMAs and exponentials wait for each
+    // other (16 heads of 128, 4096 x 16384: 656 us, in turn 535 us).
+    const int m = warp - LY::kMmaWarp, wg0 = 2 * m;  // its first warpgroup
     constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
     const bool leader = ptx::elect_one();
     const uint32_t id_s = ptx::make_idesc(1, fmt, N);
@@ -489,11 +491,21 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     } else {
       bool have = next_tile(0);
       if (have)
-        for (int wg = 0; wg < active; ++wg) load_q(it, wg);
+        for (int wg = wg0; wg < min(active, wg0 + 2); ++wg) load_q(it, wg);
       int i = 0;
       while (have && ok) {  // an item begins: its Q is on its way
-        const int cur_active = active;
-        for (int wg = 0; wg < cur_active; ++wg)
+        const int end = min(active, wg0 + 2);  // of its warpgroups with rows
+        if (end <= wg0) {  // none: keep step with the tiles
+          const bool ends = last;
+          if (leader) ptx::mbar_arrive(k_empty + 8 * (i % NS));
+          if (!wait(v_full + 8 * (i % NS), i / NS)) break;
+          if (leader) ptx::mbar_arrive(v_empty + 8 * (i % NS));
+          have = next_tile(++i);
+          if (have && ends)
+            for (int wg = wg0; wg < min(active, wg0 + 2); ++wg) load_q(it, wg);
+          continue;
+        }
+        for (int wg = wg0; wg < end; ++wg)
           if (wait(q_full + 8 * wg, q_loads[wg] - 1)) scores(i, wg);
         commit(k_empty + 8 * (i % NS));
         bool first = true, ends = false;
@@ -504,7 +516,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
           // items in between are read by the softmax only when this item's O is complete.
           if (!ends) next_tile(i);
           if (!wait(v_ready + 8 * at, cur / NS)) break;
-          for (int wg = 0; wg < cur_active; ++wg) {
+          for (int wg = wg0; wg < end; ++wg) {
             if (!product(cur, wg, first)) break;
             if (ends) commit(o_full + 8 * wg);
             else scores(i, wg);
@@ -518,7 +530,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         have = next_tile(i);
         // the next item's Q: this one's scores are done, and where Q is O's way out, O has left it
         if (have)
-          for (int wg = 0; wg < active; ++wg) {
+          for (int wg = wg0; wg < min(active, wg0 + 2); ++wg) {
             if (!LY::kOutBeside && q_loads[wg] && !wait(q_empty + 8 * wg, q_loads[wg] - 1)) break;
             load_q(it, wg);
           }
@@ -526,8 +538,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     }
     // what is in flight ends before tensor memory and shared memory are given up
     __syncwarp();
-    commit(base + LY::kDrain);
-    drain_bar(base + LY::kDrain, 0, wc);
+    commit(base + LY::kDrain + 8 * m);
+    drain_bar(base + LY::kDrain + 8 * m, 0, wc);
     for (int wg = 0; wg < WG; ++wg)
       if (q_loads[wg]) drain_bar(q_full + 8 * wg, (q_loads[wg] - 1) & 1u, wc);
   } else if (warp == LY::kFixWarp) {
