@@ -4,32 +4,48 @@
 // For query row i of a sequence and its kept states j: s_ij = scale q_i k_j, m = max s, p = exp(s -
 // m), out_i = sum p v / sum p, lse_i = m + log sum p; without kept states out = 0, lse = -inf.
 //
-// Rows: the queries of one kv head, token by token, the heads of its group side by side, so that
-// grouped heads fill an MMA's 128 rows together and read each state once: a tile is as many whole
-// tokens as fit. (Groups of more than 128 heads are cut into equal parts that read the states each
-// for itself.) Q comes and O goes as TMA boxes of such a tile; what lies behind the last token reads
-// as zeros and is not written. States come in tiles of 128. Per tile: S[128 rows, 128 states] = Q K^T
-// into tensor memory; each softmax thread owns a row, reads its 128 scores, writes the rounded
-// probabilities back as the A operand; O[128, D] += P V accumulates in tensor memory. The running
-// maximum is followed lazily: O and the row's sum are rescaled only when it has grown by more than
-// 2^8 (probabilities up to 2^8 are as exact as those up to 1, and the sums are fp32), so that most
-// tiles touch O only through the MMA.
+// Rows: the queries of one kv head, token by token, the heads of its group side by side, so
+// that grouped heads fill an MMA's 128 rows together and read each state once: a tile is as
+// many whole tokens as fit. (Groups of more than 128 heads are cut into equal parts that read
+// the states each for itself.) Q comes and O goes as TMA boxes of such a tile; what lies behind
+// the last token reads as zeros and is not written. Per tile of states: S[128 rows, states] = Q
+// K^T into tensor memory; each softmax thread owns a row, reads its scores, writes the rounded
+// probabilities back as the A operand; O[128, D] += P V accumulates in tensor memory. The
+// running maximum is followed lazily: O and the row's sum are rescaled only when it has grown
+// by more than 2^8 (probabilities up to 2^8 are as exact as those up to 1, and the sums are
+// fp32), so that most tiles touch O only through the MMA. The probabilities are summed as
+// computed and rounded once, to the inputs' type, for the product, beside the output's own
+// rounding.
 //
-// Two softmax warpgroups alternate, so that one's exponentials overlap the other's MMAs:
-//   PAIRED = false  two tiles of 128 rows per item, each state tile used by both (many rows); a CTA
-//                   takes items (sequence, kv head, 256 rows) in turn, and the loads and first scores
-//                   of the next item overlap the end of the last;
-//   PAIRED = true   one tile of rows, the warpgroups take the even and the odd state tiles (few
-//                   rows: single tokens, grouped heads), and their halves are joined at the end.
-// A cluster of CTAs may split the states of one item; the parts (fp32 O, maximum, sum) are joined
-// through distributed shared memory, every CTA finishing a share of the rows: no second launch, no
-// workspace, and the order of the sums is fixed.
+// Softmax warpgroups share the state tiles, so that the exponentials of some overlap the MMAs
+// of the others:
+//   PAIRED = false  two tiles of 128 rows per item and tiles of 128 states, or, for heads of up to
+//                   64 elements, four and 64: S and O of all of them fill tensor memory either way
+//                   (300 queries x 5456 states, heads of 32, 32 images: four warpgroups 260 us, two
+//                   297 us). A CTA takes items (sequence, group, rows) in turn;
+//   PAIRED = true   one tile of rows, two warpgroups take the even and the odd state tiles (few
+//                   rows: some tokens, grouped heads), and their halves are joined at the end.
+// A cluster of CTAs may split the states of one item; the parts (fp32 O, maximum, sum) are
+// joined through distributed shared memory, every CTA finishing a share of the rows: no second
+// launch, no workspace, and the order of the sums is fixed.
 //
-// Roles (384 threads): warps 0-3 and 4-7 softmax and epilogue, warp 8 producer (kept-state words of
-// each tile, TMA of K and V; tiles without a kept state are left out altogether), warp 9
-// issues the MMAs (and loads Q), warp 10 zeroes the V rows of states that are not kept (their
-// probability is 0, but 0 * NaN is not). Warps whose rows lie behind the last
-// query skip their exponentials. Every wait is bounded.
+// Roles: the softmax warpgroups (which also finish the rows), then a warp each for: the
+// producer (kept-state words of each tile, TMA of K and V; tiles without a kept state are left
+// out altogether), zeroing the V rows of states that are not kept (their probability is 0, but
+// 0 * NaN is not), and one or two issuers of MMAs (and of the loads of Q). Warps whose rows lie
+// behind the last query skip their exponentials. Every wait is bounded.
+//
+// Bound: at heads of 128, two row tiles times 128 states take 2756 cycles of MMAs (S, both
+// operands from shared memory: 102 cycles per 128 x 128 x 16; P V: 70) and 2048 of exponentials
+// (16 per clock and SM), and the chain of one row tile S -> P -> O -> next S takes 3250;
+// measured about 3680: 16 heads, 4096 x 16384: 486-535 us, 1.03-1.13 PFLOP/s, tensor pipe and
+// exponentials 56 % busy each. At heads of 32 the MMAs are a quarter of that and the softmax's
+// instructions and its chain set the time (260 us above: exponential unit 44 % busy, issue
+// slots 46 %).
+// Tried and slower: a polynomial on the FMA units for 1/8 to 3/8 of the exponentials (575 ->
+// 622-644 us: the issue slots are scarce too), one issuer per warpgroup at heads of 128 (656
+// us: they fall into step), scores a tile ahead with the probabilities beside them (heads of
+// 128: 535 -> 548 us, heads of 32: 297 -> 359 us).
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -94,8 +110,7 @@ struct AttnLayout {
   static constexpr int kQTiles = PAIRED ? 1 : kWGs;
   static constexpr int kStages = DP == 128 ? (PAIRED ? 3 : 2) : 6;
   static constexpr int kInfos = kStages + 2;
-  // O on its way out: beside Q, so that the next item's Q can come early, or, where shared memory
-  // is short, over it
+  // O on its way out: beside Q, or, where shared memory is short, over it
   static constexpr bool kOutBeside = !PAIRED && DP == 64;
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kK = kQTiles * kTileBytes;
@@ -113,7 +128,7 @@ struct AttnLayout {
   static constexpr uint32_t kPart = kK;
   static constexpr uint32_t kPartBytes = kAttnTile * DP * 4;
   static_assert(kPart + kWGs * kPartBytes <= kInfo, "parts fit over K, V and O");
-  static constexpr uint32_t kShare = kQ + kWGs * kAttnTile * 8;   // [row][part] factors, behind these
+  static constexpr uint32_t kShare = kQ + kWGs * kAttnTile * 8;  // [row][part] factors, behind
   static_assert(kShare + kQTiles * kAttnTile * (PAIRED ? 2 : 1) * kAttnMaxSplit * 4 <= kK,
                 "statistics and shares fit over Q");
 };
@@ -189,7 +204,6 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     return max(0, min(args.tile_tokens, left)) * args.heads;
   };
 
-  ptx::griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       ptx::mbar_init(k_full + 8 * i, 1);
@@ -217,6 +231,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     ptx::tmem_alloc(ptx::smem_addr(slot), 512);
     ptx::tmem_relinquish();
   }
+  // (not before tensor memory is taken, which a kernel that starts behind this one may want too)
+  ptx::griddep_launch_dependents();
   // the setup above overlaps the tail of the kernel ahead; memory is touched only from here
   ptx::griddep_wait();
   if (threadIdx.x == 0) *wc.err = 0;
@@ -268,11 +284,16 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / args.split);
       int t = static_cast<int>(static_cast<int64_t>(tiles) * rank / args.split);
       const uint8_t* mask = args.key_mask ? args.key_mask + it.b * args.mask_sb : nullptr;
-      uint8_t next[NW];  // the lane's mask bytes of tile t
+      // The mask is read kAhead words (256 states) at a time, the next ones on their way, so that runs
+      // of tiles without a kept state pass at a few hundred cycles per load, not per tile.
+      constexpr int kAhead = 8;
+      uint8_t next[kAhead];              // the lane's bytes
+      uint32_t words[kAhead] = {};
+      int left_words = 0;
       auto fetch = [&](int tile) {
 #pragma unroll
-        for (int x = 0; x < NW; ++x) {
-          const int j = tile * N + x * 32 + lane;
+        for (int x = 0; x < kAhead; ++x) {
+          const int64_t j = static_cast<int64_t>(tile) * N + x * 32 + lane;
           next[x] = tile < t1 && j < len ? __ldg(mask + j) : 0;
         }
       };
@@ -287,9 +308,18 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
             }
             return t++;
           }
+          if (left_words == 0) {
 #pragma unroll
-          for (int x = 0; x < NW; ++x) word[x] = __ballot_sync(0xffffffffu, next[x] != 0);
-          fetch(t + 1);
+            for (int x = 0; x < kAhead; ++x)
+              words[x] = __ballot_sync(0xffffffffu, next[x] != 0);
+            left_words = kAhead;
+            fetch(t + kAhead / NW);
+          }
+#pragma unroll
+          for (int x = 0; x < NW; ++x) word[x] = words[x];
+#pragma unroll
+          for (int x = 0; x + NW < kAhead; ++x) words[x] = words[x + NW];
+          left_words -= NW;
           uint32_t some = 0;
 #pragma unroll
           for (int x = 0; x < NW; ++x) some |= word[x];
@@ -334,7 +364,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
               for (int x = 0; x < LY::kBlocks; ++x)
                 ptx::tma_load_4d(base + LY::kV + s * LY::kStateBytes + x * LY::kStateBlock,
                                  &tmap_v, x * 64, tile * N,
-                                 (it.g / args.kv_parts) * args.v_head, it.b * args.v_batch, v_full + 8 * s);
+                                 (it.g / args.kv_parts) * args.v_head, it.b * args.v_batch,
+                                 v_full + 8 * s);
               k_ahead = false;
             }
           }
@@ -370,11 +401,11 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     }
   } else if (warp >= LY::kMmaWarp && warp < LY::kMmaWarp + LY::kIssuers) {
     // ------------------------------------------------------------ MMA issuer
-    // The warp runs this code as a whole, one elected lane issues. As little as possible stands between
-    // the arrival of probabilities and the MMAs they release: what the next tile is, and that its K is
-    // there, is found out while the softmax works. One issuer serves two warpgroups in turn, which
+    // The warp runs this code as a whole, one elected lane issues. As little as possible stands
+    // between the arrival of probabilities and the MMAs they release: what the next tile is, and
+    // that its K is there, is found out while the softmax works. One issuer serves two warpgroups in turn, which
     // keeps them apart: with one each they fall into step, and MMAs and exponentials wait for each
-    // other (16 heads of 128, 4096 x 16384: 656 us, in turn 535 us).
+    // other.
     const int m = warp - LY::kMmaWarp, wg0 = 2 * m;  // its first warpgroup
     constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
     const bool leader = ptx::elect_one();
@@ -512,8 +543,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         while (ok && !ends) {
           const int cur = i++, at = cur % NS;
           ends = last;
-          // Behind an item's end the next tile is looked for after the products: the entries of empty
-          // items in between are read by the softmax only when this item's O is complete.
+          // Behind an item's end the next tile is looked for after the products: the entries of
+          // empty items in between are read by the softmax only when this item's O is complete.
           if (!ends) next_tile(i);
           if (!wait(v_ready + 8 * at, cur / NS)) break;
           for (int wg = wg0; wg < end; ++wg) {
@@ -783,9 +814,9 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       ptx::tc_fence_before();
       ptx::cluster_sync();
       {
-        // This CTA finishes a block of the item's rows: first every row's share of each part (part y: of
-        // CTA y, or of warpgroup y % 2 of CTA y / 2), then 4 elements per thread, the loads of all
-        // parts in flight at once and a warp's in one row.
+        // This CTA finishes a block of the item's rows: first every row's share of each part (part
+        // y: of CTA y, or of warpgroup y % 2 of CTA y / 2), then 4 elements per thread, the loads
+        // of all parts in flight at once and a warp's in one row.
         constexpr int MP = PAIRED ? 2 * kAttnMaxSplit : kAttnMaxSplit;
         const Item it = item_at(item0);
         const int parts = PAIRED ? 2 * args.split : args.split;

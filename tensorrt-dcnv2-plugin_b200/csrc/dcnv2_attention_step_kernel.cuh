@@ -1,16 +1,23 @@
 // dcnv2_attention_step_kernel.cuh — attention of few query rows (single tokens and their grouped
 // heads, up to 16 per kv head) to the states of another sequence.
 //
-// The formulas are those of dcnv2_attention_kernel.cuh. Here every state is read once and used by 16
-// rows at most, so the time is that of reading K and V; the work on them only has to keep up. Each
-// warp runs by itself: it copies chunks of K and V rows (cp.async, 16 bytes per lane, 16 KB of D = 128
-// elements in flight per stage of a warp pair of chunks) into a ring of its own in shared memory,
-// multiplies with m16n8k16 MMAs on 16 padded rows, and keeps its own maximum, sum and O in
-// registers, so that no barrier stands between the loads. Tensor-memory MMAs would need 128 rows
-// (or the states as rows) and barriers between the roles; at these sizes the tensor core is idle
-// most of the time either way. The warps' parts are joined in shared memory; the CTAs of a cluster,
-// which split the states, send theirs to the CTA that finishes the element (stores into distributed
-// shared memory, one barrier), which adds them in a fixed order.
+// The formulas are those of dcnv2_attention_kernel.cuh. Here every state is read once and used
+// by 16 rows at most, so the time is that of reading K and V; the work on them only has to keep
+// up. Each warp runs by itself: it copies chunks of 4 KB of K and of V (cp.async, 16 bytes per
+// lane, two chunks ahead) into a ring of its own in shared memory, multiplies with m16n8k16
+// MMAs on 16 padded rows, and keeps its own maximum, sum and O in registers, so that no barrier
+// stands between the loads. (Tensor-memory MMAs would need 128 rows and barriers between the
+// roles: the tiled kernel takes 354 us for the 200 us below.) The warps' parts are joined in
+// shared memory; the CTAs of a cluster, which split the states, send theirs to the CTA that
+// finishes the element (stores into distributed shared memory, one barrier), which adds them in
+// a fixed order.
+//
+// Bound: HBM; a CTA draws at most about 50 GB/s, whatever it has in flight (64 to 192 KB
+// measured), so all SMs have to take part. 8 sequences of up to 60001 states, 8 kv heads of 128
+// (1.17 GB): 200 us, 5.8 TB/s, 89 % of the copy rate. 32 padded images, heads of 32: 32 us, 3.5
+// TB/s: one CTA per (image, head), the time that of the fullest image. One sequence, 8 kv
+// heads, 5456 states: 10.9 us, of which 4.3 us are a launch without states and 2 us the join
+// over 16 CTAs.
 //
 // States that are not kept are not read: their rows in shared memory are filled with zeros (the
 // copy's source size is 0), their scores are -inf; chunks without a kept state cost nothing.

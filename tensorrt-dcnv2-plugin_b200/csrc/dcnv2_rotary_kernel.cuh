@@ -21,7 +21,12 @@
 // hardware's sine and cosine (absolute error at most 2^-21.1 on [-pi, pi], beside the half step of
 // 2^-9 or 2^-12 of the output). Everything else is fp32, rounded once.
 //
-// Bound: HBM (every element read once and written once).
+// Bound: HBM (every element read once and written once) until the instructions count: a lane's head
+// costs about 280 of them per warp (16 elements: unpacking, norm, gains, rotation, packing, and its
+// share of addresses and cosines), which fill 58 % of the issue slots. Measured: 128 x 128 maps of 40
+// heads of 128, batch 4: 291 us, 4.6 TB/s, 71 % of the copy rate; keys of 5456 tokens, 8 heads of 32,
+// batch 32: 45 us, 4.0 TB/s; heads of 80 leave 3 of 8 lanes idle: 46 us, 3.2 TB/s. One to four heads
+// per lane and 8 to 32 warps per SM were measured; two and 16 are fastest.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
