@@ -242,10 +242,11 @@ typedef struct {
  * freqs[p]: out[e0] = y[e0] cos a - y[e1] sin a, out[e1] = y[e1] cos a + y[e0] sin a; the other
  * elements are y. One axis is a text, two a feature map (row, column), three a video or the levels
  * of a pyramid. fp32 arithmetic (angles reduced in fp64), one rounding.
- *   positions  int32 [batch][tokens][axes], any values; freqs  fp32 [rotary_dim/2] (both may be
- *   NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL (ones;
+ *   positions  int32 [batch][tokens][axes], any values; freqs  fp32 [rotary_dim/2], finite (both
+ *   may be NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL (ones;
  *   read only with DCNV2_NORM_RMS).
- * An output may be its own input (same pointer and strides); other overlaps are not supported.
+ * An output may be its own input (same pointer and strides); other overlaps are not supported, and
+ * an output whose strides lay rows over one another is refused.
  * Works at any element alignment, fastest where pointers, strides and dims allow 16-byte accesses.
  * All pointers are device pointers of the current device. Asynchronous on `stream`; needs no
  * workspace; batch or tokens 0 is a no-op. No counterpart in the reference plugin. */
@@ -257,14 +258,16 @@ DCNV2_API dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const
 
 /* Attention of q_tokens queries to kv_tokens states of another sequence. Strides are in elements,
  * in the order batch, token, head, multiples of 8; the elements of a head are contiguous. A batch
- * or head stride of 0 in k and v shares those states. */
+ * or head stride of 0 in k and v shares those states, a batch stride of 0 in q the queries; the rows of
+ * out may not meet. */
 typedef struct {
   int32_t batch, q_tokens, kv_tokens;
   int32_t q_heads, kv_heads;     /* q_heads a multiple of kv_heads: query head h reads kv head
                                     h / (q_heads / kv_heads) */
   int32_t head_dim;              /* a multiple of 8, at most 128 */
   int32_t dtype;                 /* DCNV2_HALF or DCNV2_BF16: q, k, v and out */
-  float scale;                   /* of the scores, > 0 (usually 1 / sqrt(head_dim)) */
+  float scale;                   /* of the scores, > 0 (usually 1 / sqrt(head_dim)) and finite, also
+                                    times log2(e) */
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
   int64_t mask_batch_stride;     /* bytes between the sequences of key_mask; 0: shared */
 } dcnv2_attention_desc;
@@ -279,7 +282,8 @@ DCNV2_API size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc
  *   kv_lens   int32 [batch] or NULL: states kept per sequence (values are clamped to
  *             [0, kv_tokens]); NULL keeps kv_tokens.
  *   key_mask  bytes [batch][kv_tokens] or NULL: state j is kept where the byte is not 0 (the pixels
- *             of a padded image). Combined with kv_lens.
+ *             of a padded image). Combined with kv_lens. Calls that need a workspace take it for at
+ *             most 2^28 states.
  *   lse       fp32 [batch][q_heads][q_tokens] or NULL: natural logarithm of the sum of the exponentials.
  * What states that are not kept hold (infinities, NaN) reaches no result. A sequence without any kept
  * state gives zeros and lse = -inf. Deterministic: the same call gives the same bits. Pointers of

@@ -62,6 +62,23 @@ bool stride_ok(int64_t stride, int64_t extent) {
   return stride >= 0 && (extent <= 1 || stride <= (int64_t(1) << 60) / extent);
 }
 
+// Whether no two rows of `width` elements of an output meet: each stride steps over all that the
+// smaller ones reach. Rows at one place would race.
+bool apart(const int64_t (&stride)[3], const int64_t (&extent)[3], int64_t width) {
+  if (!extent[0] || !extent[1] || !extent[2]) return true;
+  bool used[3] = {extent[0] == 1, extent[1] == 1, extent[2] == 1};
+  int64_t reach = width;
+  for (;;) {
+    int next = -1;
+    for (int j = 0; j < 3; ++j)
+      if (!used[j] && (next < 0 || stride[j] < stride[next])) next = j;
+    if (next < 0) return true;
+    if (stride[next] < reach) return false;
+    used[next] = true;
+    reach += stride[next] * (extent[next] - 1);
+  }
+}
+
 dcnv2_status check_rotary(const dcnv2_rotary_desc* d) {
   if (!d) return DCNV2_ERR_INVALID_ARG;
   if (!rotary_elem_bytes(d->dtype)) return DCNV2_ERR_UNSUPPORTED;
@@ -92,10 +109,9 @@ dcnv2_status check_rotary(const dcnv2_rotary_desc* d) {
     for (int j = 0; j < 3; ++j) {
       if (!stride_ok(in[i][j], extent[j]) || !stride_ok(out[i][j], extent[j]))
         return DCNV2_ERR_INVALID_ARG;
-      // outputs of two rows at one place would race
-      if (extent[j] > 1 && out[i][j] < d->head_dim && d->batch && d->tokens)
-        return DCNV2_ERR_INVALID_ARG;
     }
+    const int64_t out_stride[3] = {out[i][0], out[i][1], out[i][2]};
+    if (!apart(out_stride, extent, d->head_dim)) return DCNV2_ERR_INVALID_ARG;
   }
   return DCNV2_OK;
 }
@@ -170,12 +186,13 @@ struct AttnPlan {
   unsigned grid = 0;
 };
 
+constexpr int kMaskTokens = 1 << 28;  // states under a key mask, tiled kernel
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
 
 // CTAs of a cluster that split the states of one item, from the time of the whole in units of a state
 // tile (about 2 us: its MMAs and exponentials for both warpgroups): waves of clusters * (tiles of a
 // CTA + start + join). An item that is not split costs no join, and one start for all items of its
-// CTA. (18 items of 8 tiles, split 8: 15 of the clusters run at once, 26 us; split 4: 13 us.)
+// CTA. (18 items of 8 tiles, split 8: 15 of the clusters run at once, 26 us; split 4: 15 us.)
 int attn_split(int64_t items, int64_t tiles) {
   // clusters of 1, 2, ... CTAs that run at once with one CTA per SM, as the GPCs of 148 SMs allow
   static constexpr int kResident[kAttnMaxSplit + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
@@ -200,7 +217,7 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
       d->q_heads % d->kv_heads || d->head_dim < 1 || d->kv_tokens > INT_MAX - 1024)
     return DCNV2_ERR_INVALID_ARG;
   if (d->head_dim % 8 || d->head_dim > 128) return DCNV2_ERR_UNSUPPORTED;
-  if (!(d->scale > 0.f && std::isfinite(d->scale))) return DCNV2_ERR_INVALID_ARG;
+  if (!(d->scale > 0.f && std::isfinite(d->scale * kLog2e))) return DCNV2_ERR_INVALID_ARG;
   const int64_t qx[3] = {d->batch, d->q_tokens, d->q_heads};
   const int64_t kx[3] = {d->batch, d->kv_tokens, d->kv_heads};
   for (int j = 0; j < 3; ++j) {
@@ -211,10 +228,8 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
     if (j > 0 && qx[j] > 1 && !d->q_stride[j]) return DCNV2_ERR_UNSUPPORTED;
     if (j == 1 && kx[j] > 1 && (!d->k_stride[j] || !d->v_stride[j])) return DCNV2_ERR_UNSUPPORTED;
     if (kx[j] > 1 && (d->k_stride[j] % 8 || d->v_stride[j] % 8)) return DCNV2_ERR_UNSUPPORTED;
-    // outputs of two rows at one place would race
-    if (qx[j] > 1 && d->out_stride[j] < d->head_dim && d->batch && d->q_tokens)
-      return DCNV2_ERR_INVALID_ARG;
   }
+  if (!apart(d->out_stride, qx, d->head_dim)) return DCNV2_ERR_INVALID_ARG;
   if (!stride_ok(d->mask_batch_stride, d->batch)) return DCNV2_ERR_INVALID_ARG;
   p->wide = d->head_dim > 64;
   const int group = d->q_heads / d->kv_heads;
@@ -265,8 +280,8 @@ bool encode_map(CUtensorMap* m, const void* p, int rank, const cuuint64_t* dims,
 }
 
 // Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x the 256 / wgs tokens
-// of a tile in the 128-byte swizzle. Axes that no step is taken along, or that share their states, have extent 1.
-// What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
+// of a tile in the 128-byte swizzle. Axes that no step is taken along, or that share their states,
+// have extent 1. What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
 bool states_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
                 const dcnv2_attention_desc& d, int wgs, int* batch_step, int* head_step) {
   const bool heads = d.kv_heads > 1 && stride[2] > 0, batch = d.batch > 1 && stride[0] > 0;
@@ -325,8 +340,8 @@ dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPl
     set[dev].store(true, std::memory_order_release);
   }
   cudaLaunchAttribute at[2];
-  const cudaLaunchConfig_t cfg =
-      launch_config(p.grid, AttnLayout<DP, PAIRED>::kThreads, smem, st, at, static_cast<unsigned>(p.split));
+  const cudaLaunchConfig_t cfg = launch_config(p.grid, AttnLayout<DP, PAIRED>::kThreads, smem, st,
+                                               at, static_cast<unsigned>(p.split));
   return launched(cudaLaunchKernelEx(&cfg, kernel, a, m.q, m.k, m.v, m.o));
 }
 
@@ -481,6 +496,9 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
     return DCNV2_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(kv_lens) | reinterpret_cast<uintptr_t>(lse)) % 4)
     return DCNV2_ERR_INVALID_ARG;
+  // a search that takes longer than the kernel's waits do (2 s; a load of mask bytes takes 1 us at
+  // most and covers 256 states)
+  if (p.grid && key_mask && d.kv_tokens > kMaskTokens) return DCNV2_ERR_UNSUPPORTED;
   if (p.grid && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 ||
                  workspace_bytes < size_t(p.grid) * sizeof(int)))
     return DCNV2_ERR_WORKSPACE;

@@ -308,8 +308,9 @@ def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
     desc, ws_bytes, index, lse_shape, nothing = _attention_plan(
         _meta(q), _meta(k), _meta(v), _meta(out), _meta(kv_lens), _meta(key_mask),
         None if scale is None else float(scale))
-    if workspace is not None and workspace.get_device() != index:
-        raise ValueError(f"dcnv2_cross_attention: workspace is not on cuda:{index}")
+    if workspace is not None and (workspace.get_device() != index or
+                                  not workspace.is_contiguous()):
+        raise ValueError(f"dcnv2_cross_attention: workspace is not a contiguous tensor on cuda:{index}")
     st = _current(index) if stream is None else None
     if st is None:
         with _on(index, stream) as st:

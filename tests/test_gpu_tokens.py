@@ -316,6 +316,24 @@ def test_attention_runs_of_empty_sequences(d, by_mask):
     assert not bool(out[gone].any()) and bool((lse[gone] == -math.inf).all())
 
 
+@pytest.mark.parametrize("L,h,g,d", [(150, 2, 2, 40), (300, 2, 2, 128), (20, 4, 2, 64)])
+def test_attention_long_masked_runs(L, h, g, d):
+    """Kept states far apart, at every place of a run of mask words, lengths that end in a run."""
+    s = 2611
+    mask = torch.zeros(6, s, dtype=torch.bool)
+    mask[0, ::257] = True
+    mask[1, 63::64] = True
+    mask[2, 1023] = mask[2, 1024] = mask[2, -1] = True
+    mask[3, :40] = mask[3, 900:1300] = True
+    mask[4, 255:257] = mask[4, 2304:] = True
+    lens = torch.tensor([2611, 2000, 2610, 1200, 2559, 0], dtype=torch.int32)
+    q, k, v = attention_inputs(6, L, s, h, g, d, BF16, L + d + 1)
+    out, lse = run_attention(q, k, v, mask=mask)
+    check_attention(out, lse, q, k, v, mask=mask)
+    out, lse = run_attention(q, k, v, lens, mask)
+    check_attention(out, lse, q, k, v, lens, mask)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, -65504.0])
 @pytest.mark.parametrize("L,h,g,d", [(1, 8, 2, 64), (200, 2, 2, 128)])
 def test_attention_unkept_states_reach_nothing(L, h, g, d, bad):
@@ -476,6 +494,11 @@ def test_refusals_on_the_device():
             q, k, k, key_mask=torch.ones(1, 8, dtype=torch.bool, device=DEV))),
         (TypeError, lambda: dcnv2_cross_attention(q, k, k, key_mask=torch.ones(1, 9, device=DEV))),
         (ValueError, lambda: dcnv2_cross_attention(q, k, k, out=q[:, :3])),
+        (ValueError, lambda: dcnv2_cross_attention(
+            q, k, k, workspace=torch.empty(1, dtype=torch.uint8, device=DEV).expand(4096))),
+        (DCNv2Error, lambda: dcnv2_cross_attention(
+            q, k, k, out=torch.empty(4096, dtype=FP16, device=DEV).as_strided(
+                q.shape, (1024, 64, 64, 1)))),
         (ValueError, lambda: dcnv2_qk_norm_rotary(None, None)),
         (TypeError, lambda: dcnv2_qk_norm_rotary(q.double(), None, norm="rms")),
         (ValueError, lambda: dcnv2_qk_norm_rotary(q, k, norm="rms")),

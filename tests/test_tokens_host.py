@@ -133,6 +133,41 @@ def test_attention_refusals(kw, status):
     assert lib.dcnv2_cross_attention_workspace_size(ctypes.byref(d)) == 0
 
 
+@pytest.mark.parametrize("strides", [
+    (256, 64, 64),        # tokens and heads in the same places
+    (768, 128, 64),       # four heads of 64 in 128
+    (512, 256, 64),       # three tokens of 256 in 512
+    (64, 384, 128),       # sequences inside a head's step, tokens inside the heads' reach
+])
+def test_outputs_over_themselves_are_refused(strides):
+    assert rotary(rotary_desc(strides={"q_out": strides})) == Status.ERR_INVALID_ARG
+    d = attention_desc(q_tokens=3, q_heads=4, strides={"out": strides})
+    assert attention(d) == Status.ERR_INVALID_ARG
+
+
+def test_outputs_in_other_orders_are_taken():
+    if torch.cuda.is_available():
+        pytest.skip("would launch")
+    for strides in ((4 * 3 * 64, 64, 3 * 64),     # heads first
+                    (64, 4 * 2 * 64, 2 * 64),     # tokens, heads, sequences
+                    (4096, 1024, 72)):            # gaps
+        assert rotary(rotary_desc(strides={"q_out": strides})) == Status.ERR_NO_DEVICE
+        d = attention_desc(q_tokens=3, q_heads=4, strides={"out": strides})
+        assert attention(d) == Status.ERR_NO_DEVICE
+    d = attention_desc(q_tokens=1, q_heads=4, strides={"out": (256, 0, 64)})  # a step never taken
+    assert attention(d) == Status.ERR_NO_DEVICE
+
+
+def test_attention_scale_and_masked_length_limits():
+    assert attention(attention_desc(scale=3e38)) == Status.ERR_INVALID_ARG  # infinite in base 2
+    long = dict(batch=1, q_tokens=200, q_heads=2, kv_heads=2, head_dim=8, kv_tokens=(1 << 28) + 1)
+    assert attention(attention_desc(**long), mask=P) == Status.ERR_UNSUPPORTED
+    if not torch.cuda.is_available():
+        assert attention(attention_desc(**long)) == Status.ERR_NO_DEVICE
+        long["kv_tokens"] -= 1
+        assert attention(attention_desc(**long), mask=P) == Status.ERR_NO_DEVICE
+
+
 def test_attention_pointer_refusals_and_no_ops():
     d = attention_desc()
     bad = Status.ERR_INVALID_ARG
