@@ -39,13 +39,14 @@
 // operands from shared memory: 102 cycles per 128 x 128 x 16; P V: 70) and 2048 of exponentials
 // (16 per clock and SM), and the chain of one row tile S -> P -> O -> next S takes 3250;
 // measured about 3680: 16 heads, 4096 x 16384: 486-535 us, 1.03-1.13 PFLOP/s, tensor pipe and
-// exponentials 56 % busy each. At heads of 32 the MMAs are a quarter of that and the softmax's
-// instructions and its chain set the time (260 us above: exponential unit 44 % busy, issue
-// slots 46 %).
+// exponentials 56 % busy each. At heads of 32 the MMAs are a quarter of that, and the issuing
+// warps' instructions (about 1150 cycles per row tile and 64 states: waits, six MMAs, commits) and
+// the softmax's set the time (260 us above: exponential unit 44 % busy, issue slots 46 %).
 // Tried and slower: a polynomial on the FMA units for 1/8 to 3/8 of the exponentials (575 ->
 // 622-644 us: the issue slots are scarce too), one issuer per warpgroup at heads of 128 (656
 // us: they fall into step), scores a tile ahead with the probabilities beside them (heads of
-// 128: 535 -> 548 us, heads of 32: 297 -> 359 us).
+// 128: 535 -> 548 us, heads of 32: 297 -> 359 us), three warpgroups with two sets of scores each
+// for heads of 32 (300 queries: 251 us, but 512 queries take 1.8 times as long).
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
