@@ -716,7 +716,12 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         if (lane == 0) ptx::mbar_arrive(p_ready + 8 * w);
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      if (!mine) continue;
+      if (!mine) {
+        // the four warps stay on one item after an abort too: one that left alone would be missing at
+        // the next item's barriers
+        if (!PAIRED && args.split == 1) ok = ptx::named_barrier_and(1 + w, 128, ok);
+        continue;
+      }
       // all products of the item are done (both warpgroups' when their parts are joined)
       if (PAIRED || any) {
         bool done = ok && wait_bar<kSuspend>(o_full + 8 * w, o_turn & 1u, wc,

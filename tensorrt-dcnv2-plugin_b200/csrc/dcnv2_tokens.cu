@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "../../include/dcnv2.h"
+#include "../../include/dcnv2_diag.h"
 #include "dcnv2_attention_kernel.cuh"
 #include "dcnv2_attention_step_kernel.cuh"
 #include "dcnv2_host.cuh"
@@ -185,6 +186,9 @@ struct AttnPlan {
   int row_tiles = 0, items = 0, split = 1;
   unsigned grid = 0;
 };
+
+// Limit of each wait of the tiled kernel; shorter ones are for tests of what happens behind it.
+std::atomic<unsigned long long> g_attn_wait_ns{kDefaultTimeoutNs};
 
 constexpr int kMaskTokens = 1 << 28;  // states under a key mask, tiled kernel
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
@@ -538,7 +542,7 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
   a.items = p.items;
   a.split = p.split;
   a.scale = d.scale;
-  a.timeout_ns = kDefaultTimeoutNs;
+  a.timeout_ns = g_attn_wait_ns.load(std::memory_order_relaxed);
   AttnMaps m;
   int out_batch = 0;
   if (!rows_map(&m.q, q, d.q_stride, d, p, &a.q_batch) ||
@@ -578,6 +582,13 @@ dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,
   }
   *code = bits;
   return bits ? DCNV2_ERR_DEVICE_TIMEOUT : DCNV2_OK;
+}
+
+dcnv2_status dcnv2_diag_set_attention_wait_limit(int32_t limit_us) {
+  if (limit_us < -1 || limit_us > static_cast<int32_t>(kDefaultTimeoutNs / 1000))
+    return DCNV2_ERR_INVALID_ARG;
+  g_attn_wait_ns.store(limit_us < 0 ? kDefaultTimeoutNs : 1000ull * limit_us);
+  return DCNV2_OK;
 }
 
 }  // extern "C"

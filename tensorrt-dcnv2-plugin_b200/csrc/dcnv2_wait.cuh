@@ -48,12 +48,14 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Wa
 }
 
 // The same wait for what a kernel itself still has in flight (copies, MMAs) before it ends or frees
-// tensor memory: an abort does not cut it short, only the time limit does.
+// tensor memory: neither an abort nor a shorter limit of the other waits cuts it short, only its own
+// limit, which no copy or MMA that still runs comes near.
+constexpr unsigned long long kDrainNs = 2000000000ull;
 __device__ __forceinline__ bool drain_bar(uint32_t bar, uint32_t parity, const WaitCtx& w) {
   const uint64_t t0 = ptx::global_timer_ns();
   for (;;) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
-    if (ptx::global_timer_ns() - t0 > w.timeout_ns) {
+    if (ptx::global_timer_ns() - t0 > kDrainNs) {
       *w.abort_flag = 1;
       atomicOr(w.err, DCNV2_DEVERR_TIMEOUT_DRAIN);
       return false;

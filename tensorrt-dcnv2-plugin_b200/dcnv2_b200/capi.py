@@ -147,6 +147,7 @@ def _load() -> ctypes.CDLL:
                                                   ctypes.POINTER(P), P, ctypes.c_size_t, P]),
         "dcnv2_diag_timeout_selftest": (ctypes.c_int, [ctypes.c_uint32,
                                                        ctypes.POINTER(ctypes.c_int32)]),
+        "dcnv2_diag_set_attention_wait_limit": (ctypes.c_int, [ctypes.c_int32]),
         "dcnv2_diag_forward_events": (ctypes.c_int, [Dp, P, P, P, P, P, P, P, ctypes.c_size_t,
                                                      ctypes.c_float, ctypes.c_float, P,
                                                      ctypes.POINTER(P), ctypes.c_int32]),
@@ -193,6 +194,7 @@ EXPORTED = (
     "dcnv2_plugin_output_shape", "dcnv2_plugin_supports_format", "dcnv2_plugin_workspace_size",
     "dcnv2_plugin_enqueue", "dcnv2_diag_timeout_selftest", "dcnv2_diag_forward_events",
     "dcnv2_diag_main_kernel", "dcnv2_diag_set_kernel_override", "dcnv2_diag_binary_arch",
+    "dcnv2_diag_set_attention_wait_limit",
 )
 
 
@@ -348,3 +350,10 @@ def cross_attention_error(desc: AttentionDesc, workspace, stream=0) -> int:
     if st not in (Status.OK, Status.ERR_DEVICE_TIMEOUT):
         raise DCNv2Error(st, "dcnv2_cross_attention_read_error")
     return int(code.value)
+
+
+def set_attention_wait_limit(limit_us: int = -1) -> None:
+    """Limit of each on-chip wait of the attention calls that follow (-1: the default of 2 s)."""
+    st = lib.dcnv2_diag_set_attention_wait_limit(int(limit_us))
+    if st != Status.OK:
+        raise DCNv2Error(st, "dcnv2_diag_set_attention_wait_limit")

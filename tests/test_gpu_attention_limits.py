@@ -1,0 +1,90 @@
+"""dcnv2_cross_attention where its bounded waits run out: a mask whose search for kept states takes far
+longer than a short limit (dcnv2_diag_set_attention_wait_limit). Every wait of the kernel ends by
+itself, so the calls return and the device stays usable."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from dcnv2_b200 import capi, dcnv2_cross_attention  # noqa: E402
+
+DEV = "cuda:0"
+S = 2 ** 25  # states under the mask: a search of tens of milliseconds
+
+# sequences, query tokens, heads, kv heads, head_dim of each form of the kernel
+FORMS = [
+    (3, 20, 4, 2, 64),     # one tile of rows, states split over a cluster
+    (3, 20, 4, 2, 128),
+    (2, 300, 2, 2, 64),    # several tiles, split
+    (2, 300, 2, 2, 128),
+    (74, 130, 4, 4, 64),   # two items per CTA, two of four warpgroups without rows
+    (37, 300, 4, 4, 128),  # two items per CTA, the second tile of rows of an item short or missing
+]
+
+
+@pytest.fixture
+def limit():
+    """Sets the limit of the attention's waits for one test, and restores the default."""
+    yield capi.set_attention_wait_limit
+    capi.set_attention_wait_limit()
+
+
+def long_call(form, first_kept):
+    """A call over S states, few of them kept: the first 64 where first_kept, else none. Sequences of
+    the first half are 64 states long. The states lie over one another (each starts 8 elements behind
+    the last), so that they take little memory."""
+    b, L, h, g, d = form
+    r = torch.Generator(DEV).manual_seed(b + L + d)
+    mem = torch.randn((S - 1) * 8 + d, generator=r, device=DEV, dtype=torch.float16)
+    k = mem.as_strided((b, S, g, d), (0, 8, 0, 1))
+    q = torch.randn(b, L, h, d, generator=r, device=DEV, dtype=torch.float16)
+    mask = torch.zeros(1, S, dtype=torch.bool, device=DEV)
+    mask[0, :64] = first_kept
+    lens = torch.full((b,), S, dtype=torch.int32, device=DEV)
+    lens[:b // 2] = 64
+    desc = capi.AttentionDesc(b, L, S, h, g, d, int(capi.DType.HALF), d ** -0.5)
+    for field, t in ((desc.q_stride, q), (desc.k_stride, k), (desc.v_stride, k),
+                     (desc.out_stride, q)):
+        field[:] = t.stride()[:3]
+    ws = torch.empty(capi.attention_workspace_size(desc), dtype=torch.uint8, device=DEV)
+    out, lse = torch.empty_like(q).fill_(7), None
+
+    def call():
+        nonlocal lse
+        _, lse = dcnv2_cross_attention(q, k, k, kv_lens=lens, key_mask=mask, return_lse=True,
+                                       out=out, workspace=ws)
+        code = capi.cross_attention_error(desc, ws.data_ptr(),
+                                          torch.cuda.current_stream().cuda_stream)
+        return out, lse, code
+
+    kk = mem.as_strided((64, d), (8, 1)).double()
+    s = q.double() @ kk.T * d ** -0.5
+    want = torch.softmax(s, -1) @ kk if first_kept else torch.zeros_like(q, dtype=torch.float64)
+    want_lse = torch.logsumexp(s, -1).transpose(1, 2) if first_kept else torch.full(
+        (b, h, L), -math.inf, dtype=torch.float64, device=DEV)
+    return call, want, want_lse
+
+
+def right(out, lse, want, want_lse):
+    """[b, h, L]: rows that hold the result. Half a step of the output and of the probabilities (2^-11
+    each, of values below 8; 64 states of at most 128 elements: the rest is below 2^-12)."""
+    tol = 8 * (2 * 2.0 ** -11 + 2.0 ** -12)
+    close = ((out.double() - want).abs() <= tol).all(-1).transpose(1, 2)
+    same = (lse.double() - want_lse).abs() <= 1e-3
+    return close & (same | (lse.double() == want_lse))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("first_kept", [True, False])
+def test_calls_return_and_say_so_when_waits_run_out(limit, form, first_kept):
+    """With a limit of 1 ms the error words are set, and with the default one the same call, made
+    behind it, is right: no warp waits for one that has given up."""
+    call, want, want_lse = long_call(form, first_kept)
+    limit(1000)
+    assert call()[2] != 0
+    limit()
+    out, lse, code = call()
+    assert code == 0
+    assert bool(right(out, lse, want, want_lse).all())
