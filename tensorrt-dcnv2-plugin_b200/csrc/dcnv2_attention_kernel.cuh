@@ -383,22 +383,21 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       } while (tile >= 0);
     }
     if (lane == 0) {
-      int end = i;
-      for (; ok && end < i + 1; ++end) {  // the end
-        ok = wait_bar<kSuspend>(k_empty + 8 * (end % NS),
-                                (static_cast<uint32_t>(end / NS) & 1u) ^ 1u, wc,
-                                DCNV2_DEVERR_TIMEOUT_PRODUCER);
-        if (!ok) break;
-        tile_flags[end % NS] = kTileEnd;
-        ptx::mbar_arrive(k_full + 8 * (end % NS));
+      const int k_tiles = i + (k_ahead ? 1 : 0);
+      int k_marks = k_tiles;             // K barriers' phases: the tiles, and the end's mark
+      if (ok && wait_bar<kSuspend>(k_empty + 8 * (i % NS),
+                                   (static_cast<uint32_t>(i / NS) & 1u) ^ 1u, wc,
+                                   DCNV2_DEVERR_TIMEOUT_PRODUCER)) {
+        tile_flags[i % NS] = kTileEnd;
+        ptx::mbar_arrive(k_full + 8 * (i % NS));
+        ++k_marks;
       }
-      // Copies in flight land before the CTA ends or its buffers are used for the parts (those of K
-      // whose place an end mark has taken have).
-      for (int x = end > NS ? end - NS : 0; x < i; ++x)
+      // Copies in flight land before the CTA ends or its buffers are used for the parts. (Only a
+      // barrier's last phase can be waited for; a copy whose place another has taken has landed.)
+      for (int x = k_marks > NS ? k_marks - NS : 0; x < k_tiles; ++x)
         drain_bar(k_full + 8 * (x % NS), static_cast<uint32_t>(x / NS) & 1u, wc);
       for (int x = i > NS ? i - NS : 0; x < i; ++x)
         drain_bar(v_full + 8 * (x % NS), static_cast<uint32_t>(x / NS) & 1u, wc);
-      if (k_ahead) drain_bar(k_full + 8 * (i % NS), static_cast<uint32_t>(i / NS) & 1u, wc);
     }
   } else if (warp >= LY::kMmaWarp && warp < LY::kMmaWarp + LY::kIssuers) {
     // ------------------------------------------------------------ MMA issuer

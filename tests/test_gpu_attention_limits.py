@@ -31,9 +31,9 @@ def limit():
     capi.set_attention_wait_limit()
 
 
-def long_call(form, first_kept):
-    """A call over S states, few of them kept: the first 64 where first_kept, else none. Sequences of
-    the first half are 64 states long. The states lie over one another (each starts 8 elements behind
+def long_call(form, first_kept, again=0):
+    """A call over S states, few of them kept: the first 64 where first_kept, else none (and of every
+    2^21 the first `again`, if any). Sequences of the first half are 64 states long. The states lie over one another (each starts 8 elements behind
     the last), so that they take little memory."""
     b, L, h, g, d = form
     r = torch.Generator(DEV).manual_seed(b + L + d)
@@ -42,6 +42,8 @@ def long_call(form, first_kept):
     q = torch.randn(b, L, h, d, generator=r, device=DEV, dtype=torch.float16)
     mask = torch.zeros(1, S, dtype=torch.bool, device=DEV)
     mask[0, :64] = first_kept
+    if again:
+        mask.view(-1, 2 ** 21)[:, :again] = True
     lens = torch.full((b,), S, dtype=torch.int32, device=DEV)
     lens[:b // 2] = 64
     desc = capi.AttentionDesc(b, L, S, h, g, d, int(capi.DType.HALF), d ** -0.5)
@@ -88,3 +90,21 @@ def test_calls_return_and_say_so_when_waits_run_out(limit, form, first_kept):
     out, lse, code = call()
     assert code == 0
     assert bool(right(out, lse, want, want_lse).all())
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_copies_in_flight_are_waited_for_once(limit, form):
+    """The issuers give up while a gap of the mask is searched; behind it the producer finds tiles again
+    and fills its buffers until a place of V stays taken, with K of that tile on its way. What is in
+    flight then lands long before the limit for that, which would take 2 s and show in the error
+    words."""
+    call, _, _ = long_call(form, True, again=4096)
+    call()
+    limit(100)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    code = call()[2]
+    end.record()
+    end.synchronize()
+    assert code and not code & 16
+    assert begin.elapsed_time(end) < 1500
