@@ -297,7 +297,9 @@ DCNV2_API dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, c
                                              void* out, float* lse, void* workspace,
                                              size_t workspace_bytes, dcnv2_stream_t stream);
 
-/* ORs the error words of the last dcnv2_cross_attention call with this desc and workspace into
+/* The waits inside the kernel are bounded (2 s each). Where one runs out, all rows of out and lse that
+ * its CTA or cluster had to write become NaN, and the error words say so.
+ * ORs the error words of the last dcnv2_cross_attention call with this desc and workspace into
  * *code (0 = none, otherwise DCNV2_DEVERR_* bits, with DCNV2_ERR_DEVICE_TIMEOUT returned) after
  * synchronising `stream`. Test and debug helper, not during a stream capture. */
 DCNV2_API dcnv2_status dcnv2_cross_attention_read_error(const dcnv2_attention_desc* desc,

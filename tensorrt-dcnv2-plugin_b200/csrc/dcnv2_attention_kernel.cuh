@@ -731,10 +731,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
                             wait_bar<kSuspend>(o_full + 8 * x, o_turn & 1u, wc,
                                                DCNV2_DEVERR_TIMEOUT_EPILOGUE));
         ++o_turn;
-        if (!__all_sync(0xffffffffu, done)) {
-          l = NAN;  // shows in the result, beside the error word
-          ok = false;
-        }
+        ok = __all_sync(0xffffffffu, done);
         ptx::tc_fence_after();
       }
       if (!PAIRED && args.split == 1) {
@@ -782,7 +779,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         ptx::fence_proxy_async_smem();
         // (after an abort the four warps leave together, behind the same item)
         ok = ptx::named_barrier_and(1 + w, 128, ok);
-        if (storer && any) {
+        if (storer && any && ok) {
           for (int x = 0; x * 64 < args.D; ++x)
             ptx::tma_store_5d(&tmap_o, out + x * kAttnBlockBytes, x * 64, 0,
                               it.tok0 + w * args.tile_tokens, it.g, it.b);
@@ -895,6 +892,26 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     __syncwarp();
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
+  }
+  if (*abort_flag) {
+    // A wait ran out: which rows were finished is not known, nor what this CTA's part of a split item
+    // lacks. All rows of its items become NaN, behind what any warp or CTA of the cluster has
+    // stored (stores of this CTA have completed, those of the others are ahead of the last cluster_sync).
+    for (int item = item0; item < args.items; item += item_step) {
+      const Item it = item_at(item);
+      int n_rows = 0;
+      for (int x = 0; x < LY::kQTiles; ++x) n_rows += rows_of(it, x);
+      for (int r = threadIdx.x; r < n_rows; r += LY::kThreads) {
+        const int tok = it.tok0 + r / args.heads, h = it.g * args.heads + r % args.heads;
+        uint16_t* o = static_cast<uint16_t*>(args.out) + it.b * args.out_sb + tok * args.out_st +
+                      h * args.out_sh;
+        for (int x = 0; x < args.D; x += 8)
+          *reinterpret_cast<uint4*>(o + x) =
+              make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);  // NaN of both types
+        if (args.lse)
+          args.lse[(static_cast<int64_t>(it.b) * args.H + h) * args.L + tok] = NAN;
+      }
+    }
   }
 }
 

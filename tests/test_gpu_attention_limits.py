@@ -108,3 +108,23 @@ def test_copies_in_flight_are_waited_for_once(limit, form):
     end.synchronize()
     assert code and not code & 16
     assert begin.elapsed_time(end) < 1500
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("first_kept,again", [(True, 0), (False, 0), (True, 4096)])
+def test_rows_whose_waits_ran_out_are_nan(limit, form, first_kept, again):
+    """No row looks like a result that it is not: not like that of a sequence without kept states, not
+    like one over a part of the states, and none is left as it was. Rows and their lse are right, or
+    NaN from end to end, and those of the sequences that were searched are NaN."""
+    call, want, want_lse = long_call(form, first_kept, again)
+    limit(100)
+    out, lse, code = call()
+    assert code
+    nan = torch.isnan(out).all(-1).transpose(1, 2) & torch.isnan(lse)
+    b = out.shape[0]
+    assert bool(nan[b // 2:].all())
+    if first_kept:
+        assert bool((nan | right(out, lse, want, want_lse))[:b // 2].all())
+    else:
+        zero = ~out.any(-1).transpose(1, 2) & (lse == -math.inf)
+        assert bool((nan | zero)[:b // 2].all())
