@@ -54,6 +54,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <climits>
+
 #include "../../include/dcnv2.h"
 #include "dcnv2_wait.cuh"
 #include "ptx_sm100.cuh"
@@ -123,7 +125,7 @@ struct AttnLayout {
   static constexpr int kNumBars = 5 * kStages + 2 * kInfos + 5 * kWGs + kIssuers;
   static constexpr uint32_t kDrain = kBars + (kNumBars - kIssuers) * 8;  // the MMA issuers' own
   static constexpr uint32_t kFlags = kBars + kNumBars * 8;        // [kStages] of the K tiles
-  static constexpr uint32_t kSlot = kFlags + kStages * 4;         // TMEM address, abort flag
+  static constexpr uint32_t kSlot = kFlags + kStages * 4;         // TMEM address, abort flag, steps
   static constexpr uint32_t kBytes = kSlot + 16;
   // at the end, over K, V and what follows: fp32 O of the warpgroups; over Q: their (maximum, sum)
   static constexpr uint32_t kPart = kK;
@@ -182,6 +184,9 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   uint32_t* infos = reinterpret_cast<uint32_t*>(smem + LY::kInfo);  // words 0-3, flags
   const WaitCtx wc{args.timeout_ns, args.err + blockIdx.x, abort_flag};
+  // Waits for the producer, which may have to search long masks without a kept state, item after item
+  volatile int* producer_steps = abort_flag + 1;
+  const WaitCtx wp{args.timeout_ns, args.err + blockIdx.x, abort_flag, producer_steps};
 
   // A cluster of `split` CTAs takes the items cluster, cluster + clusters, ... (one item each when
   // split or PAIRED); item = (sequence * groups + group) * row_tiles + row tile.
@@ -225,7 +230,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       ptx::mbar_init(o_full + 8 * i, 1);
     }
     for (int i = 0; i < LY::kIssuers; ++i) ptx::mbar_init(base + LY::kDrain + 8 * i, 1);
-    *abort_flag = 0;
+    *abort_flag = *producer_steps = 0;
     ptx::fence_mbar_init();
   }
   if (warp == LY::kMmaWarp) {
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
   // Reads entry n of the producer's ring: words of the tile and flags. False after an abort.
   auto read_info = [&](int n, uint32_t (&word)[NW], uint32_t& flags, int code) {
     const bool ok = wait_bar<kSuspend>(info_full + 8 * (n % NI),
-                                       static_cast<uint32_t>(n / NI) & 1u, wc, code);
+                                       static_cast<uint32_t>(n / NI) & 1u, wp, code);
     if (!__all_sync(0xffffffffu, ok)) return false;
     const uint4 f = ptx::ld_shared_v4(base + LY::kInfo + (n % NI) * 32);
     word[0] = f.x;
@@ -274,6 +279,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
   if (warp == LY::kProducerWarp) {
     // ------------------------------------------------------------ producer
     int n = 0, i = 0;                    // ring entries, tiles
+    uint32_t fetches = 0;                // of masks
+    uint32_t steps = 0;                  // lane 0: what it has told the waiting ones
     uint32_t skipped = 0;                // items without a tile since the last one with tiles
     volatile uint32_t* tile_flags = reinterpret_cast<volatile uint32_t*>(smem + LY::kFlags);
     bool ok = true, k_ahead = false;     // k_ahead: K of tile i was started, V was not
@@ -288,6 +295,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       // The mask is read kAhead words (256 states) at a time, the next ones on their way, so that runs
       // of tiles without a kept state pass at a few hundred cycles per load, not per tile.
       constexpr int kAhead = 8;
+      constexpr uint32_t kStepFetches = (1u << 24) / (32 * kAhead);  // 2^24 states: about 25 ms
       uint8_t next[kAhead];              // the lane's bytes
       uint32_t words[kAhead] = {};
       int left_words = 0;
@@ -314,6 +322,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
             for (int x = 0; x < kAhead; ++x)
               words[x] = __ballot_sync(0xffffffffu, next[x] != 0);
             left_words = kAhead;
+            if (++fetches % kStepFetches == 0 && lane == 0) *producer_steps = ++steps & INT_MAX;
             fetch(t + kAhead / NW);
           }
 #pragma unroll
@@ -345,6 +354,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
 #pragma unroll
             for (int x = 0; x < NW; ++x) f[x] = word[x];
             f[4] = flags;
+            *producer_steps = ++steps & INT_MAX;
             ptx::mbar_arrive(info_full + 8 * at);
             if (tile >= 0)
               ok = wait_bar<kSuspend>(k_empty + 8 * s, ph ^ 1u, wc,
@@ -422,8 +432,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     const uint32_t v_hi = static_cast<uint32_t>(v_desc >> 32);
     bool ok = true;
     uint32_t q_loads[WG] = {}, p_turn[WG] = {};
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      const bool got = wait_bar(bar, parity & 1u, wc, DCNV2_DEVERR_TIMEOUT_MMA);
+    auto wait = [&](uint32_t bar, uint32_t parity, bool producer = false) {
+      const bool got = wait_bar(bar, parity & 1u, producer ? wp : wc, DCNV2_DEVERR_TIMEOUT_MMA);
       return ok = __all_sync(0xffffffffu, ok && got);
     };
     auto commit = [&](uint32_t bar) {
@@ -447,7 +457,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     bool begun = false, fresh = true, last = true;
     int active = 0;  // warpgroups with rows of the item
     auto next_tile = [&](int i) {
-      if (!wait(k_full + 8 * (i % NS), i / NS)) return false;
+      if (!wait(k_full + 8 * (i % NS), i / NS, true)) return false;
       const uint32_t flags = ptx::ld_shared_u32_volatile(base + LY::kFlags + (i % NS) * 4);
       fresh = last;
       last = (flags & kInfoLast) != 0;

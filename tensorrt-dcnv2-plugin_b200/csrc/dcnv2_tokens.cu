@@ -190,7 +190,9 @@ struct AttnPlan {
 // Limit of each wait of the tiled kernel; shorter ones are for tests of what happens behind it.
 std::atomic<unsigned long long> g_attn_wait_ns{kDefaultTimeoutNs};
 
-constexpr int kMaskTokens = 1 << 28;  // states under a key mask, tiled kernel
+// States under a key mask, tiled kernel: the search of a longer row without a kept state would hold an
+// SM for more than 0.46 s per item.
+constexpr int kMaskTokens = 1 << 28;
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
 
 // CTAs of a cluster that split the states of one item, from the time of the whole in units of a state
@@ -500,8 +502,6 @@ dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void*
     return DCNV2_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(kv_lens) | reinterpret_cast<uintptr_t>(lse)) % 4)
     return DCNV2_ERR_INVALID_ARG;
-  // a search that takes longer than the kernel's waits do (2 s; a load of mask bytes takes 1 us at
-  // most and covers 256 states)
   if (p.grid && key_mask && d.kv_tokens > kMaskTokens) return DCNV2_ERR_UNSUPPORTED;
   if (p.grid && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4 ||
                  workspace_bytes < size_t(p.grid) * sizeof(int)))

@@ -16,17 +16,22 @@ namespace dcnv2 {
 // the thread until the phase completes; 0 spins (the MMA issuer, whose wake-up latency is on the
 // critical path). Waiting warps that do not spin leave the issue slots to the working ones.
 // CL selects a cluster-scope acquire (barriers that the peer CTA of a pair arrives on).
+// Where the wait is for a role whose own work may take long, `moved` is a count that this role steps
+// as it gets on: the time limit starts again, once, and then whenever the count has changed (it is
+// read only when the limit is over, so that a wait that ends in time costs nothing more).
 constexpr int kSuspend = -1;
 struct WaitCtx {
   unsigned long long timeout_ns;
   int* err;                  // device error word
   volatile int* abort_flag;  // this CTA's abort flag (shared memory)
+  volatile int* moved = nullptr;
 };
 template <int SLEEP_NS = 0, bool CL = false>
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const WaitCtx& w,
                                          int code) {
   if (CL ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = ptx::global_timer_ns();
+  uint64_t t0 = ptx::global_timer_ns();
+  int seen = -1;  // (counts are not negative)
   for (uint32_t n = 1;; ++n) {
     if constexpr (SLEEP_NS > 0) __nanosleep(static_cast<unsigned>(SLEEP_NS));
     if constexpr (CL) {
@@ -39,6 +44,14 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Wa
     if ((n & 15u) == 0) {
       if (*w.abort_flag) return false;
       if (ptx::global_timer_ns() - t0 > w.timeout_ns) {
+        if (w.moved) {
+          const int now = *w.moved;
+          if (now != seen) {
+            seen = now;
+            t0 = ptx::global_timer_ns();
+            continue;
+          }
+        }
         *w.abort_flag = 1;
         atomicOr(w.err, code);
         return false;

@@ -31,9 +31,9 @@ def limit():
     capi.set_attention_wait_limit()
 
 
-def long_call(form, first_kept, again=0):
+def long_call(form, first_kept, again=0, short=True):
     """A call over S states, few of them kept: the first 64 where first_kept, else none (and of every
-    2^21 the first `again`, if any). Sequences of the first half are 64 states long. The states lie over one another (each starts 8 elements behind
+    2^21 the first `again`, if any). Sequences of the first half are 64 states long, if `short`. The states lie over one another (each starts 8 elements behind
     the last), so that they take little memory."""
     b, L, h, g, d = form
     r = torch.Generator(DEV).manual_seed(b + L + d)
@@ -45,7 +45,8 @@ def long_call(form, first_kept, again=0):
     if again:
         mask.view(-1, 2 ** 21)[:, :again] = True
     lens = torch.full((b,), S, dtype=torch.int32, device=DEV)
-    lens[:b // 2] = 64
+    if short:
+        lens[:b // 2] = 64
     desc = capi.AttentionDesc(b, L, S, h, g, d, int(capi.DType.HALF), d ** -0.5)
     for field, t in ((desc.q_stride, q), (desc.k_stride, k), (desc.v_stride, k),
                      (desc.out_stride, q)):
@@ -128,3 +129,15 @@ def test_rows_whose_waits_ran_out_are_nan(limit, form, first_kept, again):
     else:
         zero = ~out.any(-1).transpose(1, 2) & (lse == -math.inf)
         assert bool((nan | zero)[:b // 2].all())
+
+
+@pytest.mark.parametrize("d,L", [(64, 130), (128, 130)])
+@pytest.mark.parametrize("first_kept", [True, False])
+def test_searches_in_a_row_do_not_add_up(limit, d, L, first_kept):
+    """Four items per CTA, each with a search of 2^25 states (about 50 ms): a limit that is above the
+    time of 2^24 of them and far below that of all does not run out, whoever waits meanwhile."""
+    call, want, want_lse = long_call((148, L, 4, 4, d), first_kept, short=False)
+    limit(80000)
+    out, lse, code = call()
+    assert code == 0
+    assert bool(right(out, lse, want, want_lse).all())
