@@ -5,12 +5,16 @@ dcnv2_qk_norm_rotary   RMS norm of each query and key head and its rotation by t
                        on one to four axes (text; row and column; frame or level, row, column)
 dcnv2_cross_attention  attention of queries to the states of another sequence: many queries or
                        single tokens, grouped heads, lengths and masks of padded images
+dcnv2_cross_attention_workspace_size, dcnv2_cross_attention_error
+                       the workspace of such a call, and the error words that it left there
 rotary_axes            frequency table and axis of each rotated pair, made once per model
 level_positions        (level, row, column) of every pixel of a pyramid's levels
 
 Both operators take strided torch CUDA tensors (views of one projection, caches laid out heads
 first), run on the current torch stream of the tensors' device unless a stream is given, and raise
-DCNv2Error on any failure. They are inference operators, as the layer is: no gradients.
+DCNv2Error when the call is refused or cannot be launched. A wait inside the attention's kernel that
+runs out later makes the rows it concerns NaN; who wants to be told keeps the workspace and reads its
+error words (dcnv2_cross_attention_error). They are inference operators, as the layer is: no gradients.
 """
 from __future__ import annotations
 
@@ -21,7 +25,7 @@ import math
 from typing import Sequence
 
 from . import capi
-from .capi import AttentionDesc, DCNv2Error, DType, Norm, RotaryDesc, lib
+from .capi import AttentionDesc, DCNv2Error, DType, Norm, RotaryDesc, Status, lib
 
 
 @functools.lru_cache(maxsize=None)
@@ -299,8 +303,9 @@ def dcnv2_cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None,
     kv_lens    int32 [batch]: kept states per sequence; None keeps all
     key_mask   bool or uint8 [batch or 1, kv_tokens]: states kept (pixels of padded images)
     scale      of the scores; None: 1 / sqrt(head_dim)
-    workspace  CUDA tensor of at least dcnv2_cross_attention_workspace_size bytes (allocated when
-               absent or too small); not shared by calls that may overlap
+    workspace  contiguous CUDA tensor of at least dcnv2_cross_attention_workspace_size(q, k, v) bytes
+               (allocated when absent or too small, and dropped with its error words); not shared by
+               calls that may overlap
     All tensors: any strides that are multiples of 8 elements, contiguous heads, 16-byte aligned;
     head_dim a multiple of 8, at most 128. A sequence without kept states gives zeros. Returns out
     [batch, q_tokens, q_heads, head_dim], or (out, lse) with lse fp32 [batch, q_heads, q_tokens]."""
@@ -341,3 +346,29 @@ def _attention_launch(desc, ws_bytes, nothing, q, k, v, kv_lens, key_mask, out, 
     if rc:
         raise DCNv2Error(rc, "dcnv2_cross_attention")
     return out, lse
+
+
+def dcnv2_cross_attention_workspace_size(q, k, v) -> int:
+    """Workspace bytes of dcnv2_cross_attention(q, k, v): one error word per CTA, or 0 when nothing in
+    the call waits (up to 16 query rows per kv head) or there is nothing to do."""
+    return _attention_plan(_meta(q), _meta(k), _meta(v), None, None, None, None)[1]
+
+
+def dcnv2_cross_attention_error(q, k, v, workspace, stream=None) -> int:
+    """Error bits (0: none) that the last dcnv2_cross_attention call with tensors of these shapes and
+    strides left in the workspace it was given, after synchronising the stream (the current one of q's
+    device unless given). Not during a stream capture."""
+    what = "dcnv2_cross_attention_error"
+    desc, ws_bytes, index, _, _ = _attention_plan(_meta(q), _meta(k), _meta(v), None, None, None, None)
+    if ws_bytes == 0:
+        return 0
+    if workspace is None or workspace.get_device() != index or not workspace.is_contiguous() or \
+            workspace.nbytes < ws_bytes:
+        raise ValueError(f"{what}: workspace is not a contiguous tensor of {ws_bytes} bytes on "
+                         f"cuda:{index}")
+    code = ctypes.c_int32(0)
+    with _on(index, stream) as st:
+        rc = lib.dcnv2_cross_attention_read_error(desc, workspace.data_ptr(), st, ctypes.byref(code))
+    if rc not in (Status.OK, Status.ERR_DEVICE_TIMEOUT):
+        raise DCNv2Error(rc, what)
+    return code.value

@@ -1,7 +1,8 @@
 """The diagnostic limit of the attention's waits, without a GPU: what it takes and refuses."""
 import pytest
+import torch
 
-from dcnv2_b200 import capi
+from dcnv2_b200 import (capi, dcnv2_cross_attention_error, dcnv2_cross_attention_workspace_size)
 from dcnv2_b200.capi import DCNv2Error, Status, lib
 
 
@@ -13,3 +14,13 @@ def test_wait_limit_range():
     with pytest.raises(DCNv2Error):
         capi.set_attention_wait_limit(-7)
     capi.set_attention_wait_limit()
+
+
+def test_workspace_helpers_refuse_what_the_call_refuses():
+    q, k = torch.zeros(1, 40, 4, 64).half(), torch.zeros(1, 9, 2, 64).half()
+    for call in (lambda: dcnv2_cross_attention_workspace_size(q, k, k),   # not on a GPU
+                 lambda: dcnv2_cross_attention_error(q, k, k, None)):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(TypeError):
+        dcnv2_cross_attention_workspace_size(q.float(), k.float(), k.float())

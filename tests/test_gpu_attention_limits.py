@@ -8,7 +8,8 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from dcnv2_b200 import capi, dcnv2_cross_attention  # noqa: E402
+from dcnv2_b200 import (capi, dcnv2_cross_attention, dcnv2_cross_attention_error,  # noqa: E402
+                        dcnv2_cross_attention_workspace_size)
 
 DEV = "cuda:0"
 S = 2 ** 25  # states under the mask: a search of tens of milliseconds
@@ -141,3 +142,31 @@ def test_searches_in_a_row_do_not_add_up(limit, d, L, first_kept):
     out, lse, code = call()
     assert code == 0
     assert bool(right(out, lse, want, want_lse).all())
+
+
+@pytest.mark.parametrize("L,h,g,d", [(20, 4, 2, 64), (300, 2, 2, 128)])
+def test_error_words_through_the_package(limit, L, h, g, d):
+    """A caller that keeps the workspace reads the error of its last call, on the stream it ran on, and
+    cannot take another tensor for it."""
+    q = torch.randn(1, L, h, d, device=DEV).half()
+    mem = torch.zeros((S - 1) * 8 + d, device=DEV, dtype=torch.float16)
+    k = mem.as_strided((1, S, g, d), (0, 8, 0, 1))
+    mask = torch.zeros(1, S, dtype=torch.bool, device=DEV)
+    size = dcnv2_cross_attention_workspace_size(q, k, k)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    assert size > 0
+    limit(100)
+    out = dcnv2_cross_attention(q, k, k, key_mask=mask, workspace=ws, stream=side.cuda_stream)
+    assert dcnv2_cross_attention_error(q, k, k, ws, stream=side.cuda_stream) != 0
+    assert bool(torch.isnan(out).all())
+    limit()
+    out = dcnv2_cross_attention(q, k, k, key_mask=mask, workspace=ws)
+    assert dcnv2_cross_attention_error(q, k, k, ws) == 0 and not bool(out.any())
+    for bad in (None, ws[1:], ws.cpu(), torch.empty(1, dtype=torch.uint8, device=DEV).expand(size)):
+        with pytest.raises(ValueError):
+            dcnv2_cross_attention_error(q, k, k, bad)
+    one = q[:, :1]
+    assert dcnv2_cross_attention_workspace_size(one, k, k) == 0
+    assert dcnv2_cross_attention_error(one, k, k, None) == 0
