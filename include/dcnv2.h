@@ -241,7 +241,7 @@ typedef struct {
  * y = norm(x); for rotated pair p of elements (e0, e1) and a = positions[b][t][pair_axis[p]] *
  * freqs[p]: out[e0] = y[e0] cos a - y[e1] sin a, out[e1] = y[e1] cos a + y[e0] sin a; the other
  * elements are y. One axis is a text, two a feature map (row, column), three a video or the levels
- * of a pyramid. fp32 arithmetic (angles reduced in fp64), one rounding.
+ * of a pyramid. fp32 arithmetic (angles reduced in 64-bit fixed point), one rounding.
  *   positions  int32 [batch][tokens][axes], any values; freqs  fp32 [rotary_dim/2], finite (both
  *   may be NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL (ones;
  *   read only with DCNV2_NORM_RMS).

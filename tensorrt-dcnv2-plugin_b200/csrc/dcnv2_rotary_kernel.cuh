@@ -16,8 +16,10 @@
 // Angles: turns = position * freq / 2 pi modulo 1 in 64-bit fixed point (the product of the position
 // and the fraction freq / 2 pi * 2^64 wraps around whole turns by itself), of which the upper 32
 // bits are the angle. In fp32 the product alone would be off by position * freq * 2^-24 radians
-// (0.006 at position 100000); here the error is that of the fp64 freq / 2 pi, position * freq *
-// 2^-54, and 2^-25 turns of the fp32 fraction. fp32 tensors take sincospif of it, 16-bit ones the
+// (0.006 at position 100000), in fp64 by position * freq * 2^-53 and more (2^-22 at position 2^31
+// and freq 1). Here freq / 2 pi is taken in two doubles, so that its fraction is right to 2^-64 turns
+// (and freq * 2^-107): the error is position times that, 2^-33 turns at most for freq below 2^42, and
+// 2^-26 turns of rounding the angle to fp32. fp32 tensors take sincospif of it, 16-bit ones the
 // hardware's sine and cosine (absolute error at most 2^-21.1 on [-pi, pi], beside the half step of
 // 2^-9 or 2^-12 of the output). Everything else is fp32, rounded once.
 //
@@ -198,9 +200,14 @@ __global__ void __launch_bounds__(kRotThreads, kRotResident / kRotWarps)
   ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   for (int p = threadIdx.x; p < args.rot_pairs; p += kRotThreads) {
-    double per = static_cast<double>(__ldg(args.freqs + p)) * 0.15915494309189533577;
-    per -= floor(per);
-    turn_table[p] = static_cast<uint64_t>(per * 18446744073709551616.0);
+    // 1 / 2 pi in two doubles; each part's whole turns are left out before it is scaled
+    constexpr double kTurnHi = 0x1.45f306dc9c883p-3, kTurnLo = -0x1.6b01ec5417056p-57;
+    const double f = __ldg(args.freqs + p);
+    double hi = f * kTurnHi, lo = fma(f, kTurnLo, fma(f, kTurnHi, -hi));
+    hi -= rint(hi);
+    lo -= rint(lo);
+    turn_table[p] = static_cast<uint64_t>(__double2ll_rn(hi * 0x1p64)) +
+                    static_cast<uint64_t>(__double2ll_rn(lo * 0x1p64));
     axis_table[p] = (args.pair_axis[p >> 4] >> (2 * (p & 15))) & 3;
   }
   __syncthreads();

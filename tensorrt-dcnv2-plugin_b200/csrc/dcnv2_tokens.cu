@@ -28,7 +28,7 @@ DevInfo* current_device(int* dev) {
 
 cudaLaunchConfig_t launch_config(unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
                                  cudaLaunchAttribute (&attr)[2], unsigned cluster) {
-  // may start while the kernel ahead of it finishes; both kernels call griddep_wait before they
+  // may start while the kernel ahead of it finishes; all three kernels call griddep_wait before they
   // touch memory
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
