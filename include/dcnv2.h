@@ -243,8 +243,8 @@ typedef struct {
  * elements are y. One axis is a text, two a feature map (row, column), three a video or the levels
  * of a pyramid. fp32 arithmetic (angles reduced in 64-bit fixed point), one rounding.
  *   positions  int32 [batch][tokens][axes], any values; freqs  fp32 [rotary_dim/2], finite (both
- *   may be NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL (ones;
- *   read only with DCNV2_NORM_RMS).
+ *   may be NULL when rotary_dim is 0); q_weight, k_weight  [head_dim] gains of the norm or NULL
+ *   (ones; read only with DCNV2_NORM_RMS).
  * An output may be its own input (same pointer and strides); other overlaps are not supported, and
  * an output whose strides lay rows over one another is refused.
  * Works at any element alignment, fastest where pointers, strides and dims allow 16-byte accesses.
@@ -258,8 +258,8 @@ DCNV2_API dcnv2_status dcnv2_qk_norm_rotary(const dcnv2_rotary_desc* desc, const
 
 /* Attention of q_tokens queries to kv_tokens states of another sequence. Strides are in elements,
  * in the order batch, token, head, multiples of 8; the elements of a head are contiguous. A batch
- * or head stride of 0 in k and v shares those states, a batch stride of 0 in q the queries; the rows of
- * out may not meet. */
+ * or head stride of 0 in k and v shares those states, a batch stride of 0 in q the queries; the
+ * rows of out may not meet. */
 typedef struct {
   int32_t batch, q_tokens, kv_tokens;
   int32_t q_heads, kv_heads;     /* q_heads a multiple of kv_heads: query head h reads kv head
@@ -284,21 +284,22 @@ DCNV2_API size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc
  *   key_mask  bytes [batch][kv_tokens] or NULL: state j is kept where the byte is not 0 (the pixels
  *             of a padded image). Combined with kv_lens. Calls that need a workspace take it for at
  *             most 2^28 states.
- *   lse       fp32 [batch][q_heads][q_tokens] or NULL: natural logarithm of the sum of the exponentials.
- * What states that are not kept hold (infinities, NaN) reaches no result. A sequence without any kept
- * state gives zeros and lse = -inf. Deterministic: the same call gives the same bits. Pointers of
- * q, k, v and out are 16-byte aligned device pointers of the current device; out overlaps no input.
- * Asynchronous on `stream`; never allocates or synchronises. The workspace needs no setting up, and
- * calls that may overlap on the GPU need one each. Single tokens and few rows split the states over
- * a thread-block cluster. No counterpart in the reference plugin. */
+ *   lse       fp32 [batch][q_heads][q_tokens] or NULL: natural logarithm of the sum of the
+ *   exponentials.
+ * What states that are not kept hold (infinities, NaN) reaches no result. A sequence without any
+ * kept state gives zeros and lse = -inf. Deterministic: the same call gives the same bits. Pointers
+ * of q, k, v and out are 16-byte aligned device pointers of the current device; out overlaps no
+ * input. Asynchronous on `stream`; never allocates or synchronises. The workspace needs no setting
+ * up, and calls that may overlap on the GPU need one each. Single tokens and few rows split the
+ * states over a thread-block cluster. No counterpart in the reference plugin. */
 DCNV2_API dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void* q,
                                              const void* k, const void* v,
                                              const int32_t* kv_lens, const uint8_t* key_mask,
                                              void* out, float* lse, void* workspace,
                                              size_t workspace_bytes, dcnv2_stream_t stream);
 
-/* The waits inside the kernel are bounded (2 s each). Where one runs out, all rows of out and lse that
- * its CTA or cluster had to write become NaN, and the error words say so.
+/* The waits inside the kernel are bounded (2 s each). Where one runs out, all rows of out and lse
+ * that its CTA or cluster had to write become NaN, and the error words say so.
  * ORs the error words of the last dcnv2_cross_attention call with this desc and workspace into
  * *code (0 = none, otherwise DCNV2_DEVERR_* bits, with DCNV2_ERR_DEVICE_TIMEOUT returned) after
  * synchronising `stream`. Test and debug helper, not during a stream capture. */

@@ -19,10 +19,10 @@ extern "C" {
  * Returns DCNV2_ERR_DEVICE_TIMEOUT (expected) with the recorded bits in *device_code. */
 DCNV2_API dcnv2_status dcnv2_diag_timeout_selftest(uint32_t timeout_us, int32_t* device_code);
 
-/* Limit in microseconds of each on-chip wait of the dcnv2_cross_attention calls that follow, process-
- * wide: 0 to 2000000, or -1 for the default (2 s). A wait beyond it gives up, the call's error words
- * say so, and the kernel returns normally: a mask whose search takes longer than a short limit
- * shows what a failed call leaves. */
+/* Limit in microseconds of each on-chip wait of the dcnv2_cross_attention calls that follow,
+ * process-wide: 0 to 2000000, or -1 for the default (2 s). A wait beyond it gives up, the call's error
+ * words say so, and the kernel returns normally: a mask whose search takes longer than a short
+ * limit shows what a failed call leaves. */
 DCNV2_API dcnv2_status dcnv2_diag_set_attention_wait_limit(int32_t limit_us);
 
 /* dcnv2_forward with a CUDA event recorded on `stream` before each of its launches and one after

@@ -15,7 +15,9 @@
 // by more than 2^8 (probabilities up to 2^8 are as exact as those up to 1, and the sums are
 // fp32), so that most tiles touch O only through the MMA. The probabilities are summed as
 // computed and rounded once, to the inputs' type, for the product, beside the output's own
-// rounding.
+// rounding: an MMA takes both operands in one type, and fp32 ones (tf32) would need V converted
+// and run at half the rate. Error against 64 bits (2-norm): bf16 0.0023, fp16 0.00029, where the
+// output's rounding alone makes 0.0017 and 0.00021.
 //
 // Softmax warpgroups share the state tiles, so that the exponentials of some overlap the MMAs
 // of the others:
@@ -33,15 +35,21 @@
 // producer (kept-state words of each tile, TMA of K and V; tiles without a kept state are left
 // out altogether), zeroing the V rows of states that are not kept (their probability is 0, but
 // 0 * NaN is not), and one or two issuers of MMAs (and of the loads of Q). Warps whose rows lie
-// behind the last query skip their exponentials. Every wait is bounded.
+// behind the last query skip their exponentials. Every wait is bounded; where one runs out, the
+// CTA's rows (the cluster's item) become NaN.
 //
 // Bound: at heads of 128, two row tiles times 128 states take 2756 cycles of MMAs (S, both
 // operands from shared memory: 102 cycles per 128 x 128 x 16; P V: 70) and 2048 of exponentials
 // (16 per clock and SM), and the chain of one row tile S -> P -> O -> next S takes 3250;
-// measured about 3680: 16 heads, 4096 x 16384: 486-535 us, 1.03-1.13 PFLOP/s, tensor pipe and
-// exponentials 56 % busy each. At heads of 32 the MMAs are a quarter of that, and the issuing
-// warps' instructions (about 1150 cycles per row tile and 64 states: waits, six MMAs, commits) and
-// the softmax's set the time (260 us above: exponential unit 44 % busy, issue slots 46 %).
+// measured about 3680: 16 heads, 4096 x 16384: 541 us, 1.02 PFLOP/s (503 at best, 555-562 with
+// inputs that change from call to call), tensor pipe and exponentials 56 % busy each; 256 items on
+// 148 SMs are two rounds for 1.73 of work. At heads of 32 the MMAs are a quarter of that, and the
+// issuing warps' instructions (about 1150 cycles per row tile and 64 states: waits, six MMAs,
+// commits) and the softmax's set the time (260 us above: exponential unit 44 % busy, issue slots 46
+// %).
+// One tile of rows (PAIRED), 32 rows of 8 kv heads of 128, 8 x 60001 states: 311 us, 6.3 TB/s;
+// 17 rows, 8 heads of 32, 32 x 5456: 85 us; 64 heads on one kv head, 8 x 60001: 81 us, 3.0 TB/s (64
+// CTAs).
 // Tried and slower: a polynomial on the FMA units for 1/8 to 3/8 of the exponentials (575 ->
 // 622-644 us: the issue slots are scarce too), one issuer per warpgroup at heads of 128 (656
 // us: they fall into step), scores a tile ahead with the probabilities beside them (heads of
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   uint32_t* infos = reinterpret_cast<uint32_t*>(smem + LY::kInfo);  // words 0-3, flags
   const WaitCtx wc{args.timeout_ns, args.err + blockIdx.x, abort_flag};
-  // Waits for the producer, which may have to search long masks without a kept state, item after item
+  // Waits for the producer, which may have to search one long mask after another
   volatile int* producer_steps = abort_flag + 1;
   const WaitCtx wp{args.timeout_ns, args.err + blockIdx.x, abort_flag, producer_steps};
 
@@ -292,8 +300,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
       const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / args.split);
       int t = static_cast<int>(static_cast<int64_t>(tiles) * rank / args.split);
       const uint8_t* mask = args.key_mask ? args.key_mask + it.b * args.mask_sb : nullptr;
-      // The mask is read kAhead words (256 states) at a time, the next ones on their way, so that runs
-      // of tiles without a kept state pass at a few hundred cycles per load, not per tile.
+      // The mask is read kAhead words (256 states) at a time, the next ones on their way, so that
+      // runs of tiles without a kept state pass at a few hundred cycles per load, not per tile.
       constexpr int kAhead = 8;
       constexpr uint32_t kStepFetches = (1u << 24) / (32 * kAhead);  // 2^24 states: about 25 ms
       uint8_t next[kAhead];              // the lane's bytes
@@ -413,9 +421,9 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     // ------------------------------------------------------------ MMA issuer
     // The warp runs this code as a whole, one elected lane issues. As little as possible stands
     // between the arrival of probabilities and the MMAs they release: what the next tile is, and
-    // that its K is there, is found out while the softmax works. One issuer serves two warpgroups in turn, which
-    // keeps them apart: with one each they fall into step, and MMAs and exponentials wait for each
-    // other.
+    // that its K is there, is found out while the softmax works. One issuer serves two warpgroups
+    // in turn, which keeps them apart: with one each they fall into step, and MMAs and exponentials
+    // wait for each other.
     const int m = warp - LY::kMmaWarp, wg0 = 2 * m;  // its first warpgroup
     constexpr uint32_t fmt = BF16 ? ptx::kFmtBf16 : 0;
     const bool leader = ptx::elect_one();
@@ -726,8 +734,8 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (!mine) {
-        // the four warps stay on one item after an abort too: one that left alone would be missing at
-        // the next item's barriers
+        // the four warps stay on one item after an abort too: one that left alone would be missing
+        // at the next item's barriers
         if (!PAIRED && args.split == 1) ok = ptx::named_barrier_and(1 + w, 128, ok);
         continue;
       }
@@ -904,9 +912,10 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
     ptx::tmem_dealloc(tmem, 512);
   }
   if (*abort_flag) {
-    // A wait ran out: which rows were finished is not known, nor what this CTA's part of a split item
-    // lacks. All rows of its items become NaN, behind what any warp or CTA of the cluster has
-    // stored (stores of this CTA have completed, those of the others are ahead of the last cluster_sync).
+    // A wait ran out: which rows were finished is not known, nor what this CTA's part of a split
+    // item lacks. All rows of its items become NaN, behind what any warp or CTA of the cluster has
+    // stored (stores of this CTA have completed, those of the others are ahead of the last
+    // cluster_sync).
     for (int item = item0; item < args.items; item += item_step) {
       const Item it = item_at(item);
       int n_rows = 0;

@@ -7,17 +7,19 @@
 // lane, two chunks ahead) into a ring of its own in shared memory, multiplies with m16n8k16
 // MMAs on 16 padded rows, and keeps its own maximum, sum and O in registers, so that no barrier
 // stands between the loads. (Tensor-memory MMAs would need 128 rows and barriers between the
-// roles: the tiled kernel takes 354 us for the 200 us below.) The warps' parts are joined in
+// roles: the tiled kernel takes 88 us where this one takes 32, for 32 x 5456 states, heads of 32;
+// at 8 x 60001 states of 8 kv heads of 128 309 and 288.) The warps' parts are joined in
 // shared memory; the CTAs of a cluster, which split the states, send theirs to the CTA that
 // finishes the element (stores into distributed shared memory, one barrier), which adds them in
 // a fixed order.
 //
 // Bound: HBM; a CTA draws at most about 50 GB/s, whatever it has in flight (64 to 192 KB
 // measured), so all SMs have to take part. 8 sequences of up to 60001 states, 8 kv heads of 128
-// (1.17 GB): 200 us, 5.8 TB/s, 89 % of the copy rate. 32 padded images, heads of 32: 32 us, 3.5
-// TB/s: one CTA per (image, head), the time that of the fullest image. One sequence, 8 kv
-// heads, 5456 states: 10.9 us, of which 4.3 us are a launch without states and 2 us the join
-// over 16 CTAs.
+// (1.17 GB): 202 us, 5.8 TB/s, 89 % of the copy rate (213 us, 5.5 TB/s, with inputs that change
+// from call to call); all 60001 of each: 288 us, 6.8 TB/s. 32 padded images, heads of 32: 32 us,
+// 3.5 TB/s: one CTA per (image, head), two on most SMs, the time that of the fullest images;
+// without padding the same 32 us are 5.6 TB/s. One sequence, 8 kv heads, 5456 states: 10.9 us, of
+// which 4.3 us are a launch without states and 2 us the join over 16 CTAs.
 //
 // States that are not kept are not read: their rows in shared memory are filled with zeros (the
 // copy's source size is 0), their scores are -inf; chunks without a kept state cost nothing.
@@ -84,7 +86,6 @@ struct StepCopy {
   const uint16_t *k, *v;   // of row r0 of the first chunk
   int64_t kst, vst;        // elements between the lane's rows
   uint32_t r0;
-  uint32_t at;             // byte offset of row r0 in a tile, without the mixing
   uint32_t c;
   bool inside;             // the piece lies inside the head
 

@@ -8,27 +8,27 @@
 // Work split: a head's D/2 pairs are cut into chunks of VEC pairs, one lane per chunk (two vector
 // loads of VEC elements), a power of two of lanes per head, so the norm is a shuffle reduction. The
 // elements behind the rotated ones are taken as pairs too (first half, second half) with cos = 1,
-// sin = 0. A team of lanes (a warp, or a power of two of its lanes when a token has few heads) takes
-// a token's heads, kRotHeads per lane and step; its lanes compute the token's cosines and sines
-// between them, once for all heads, into shared memory. Every team takes an equal run of
+// sin = 0. A team of lanes (a warp, or a power of two of its lanes when a token has few heads)
+// takes a token's heads, kRotHeads per lane and step; its lanes compute the token's cosines and
+// sines between them, once for all heads, into shared memory. Every team takes an equal run of
 // neighbouring tokens (or, with few tokens, a part of a token's heads) and loads a step ahead.
 //
-// Angles: turns = position * freq / 2 pi modulo 1 in 64-bit fixed point (the product of the position
-// and the fraction freq / 2 pi * 2^64 wraps around whole turns by itself), of which the upper 32
-// bits are the angle. In fp32 the product alone would be off by position * freq * 2^-24 radians
-// (0.006 at position 100000), in fp64 by position * freq * 2^-53 and more (2^-22 at position 2^31
-// and freq 1). Here freq / 2 pi is taken in two doubles, so that its fraction is right to 2^-64 turns
-// (and freq * 2^-107): the error is position times that, 2^-33 turns at most for freq below 2^42, and
-// 2^-26 turns of rounding the angle to fp32. fp32 tensors take sincospif of it, 16-bit ones the
-// hardware's sine and cosine (absolute error at most 2^-21.1 on [-pi, pi], beside the half step of
-// 2^-9 or 2^-12 of the output). Everything else is fp32, rounded once.
+// Angles: turns = position * freq / 2 pi modulo 1 in 64-bit fixed point (the product of the
+// position and the fraction freq / 2 pi * 2^64 wraps around whole turns by itself), of which the
+// upper 32 bits are the angle. In fp32 the product alone would be off by position * freq * 2^-24
+// radians (0.006 at position 100000), in fp64 by position * freq * 2^-53 and more (2^-22 at
+// position 2^31 and freq 1). Here freq / 2 pi is taken in two doubles, so that its fraction is
+// right to 2^-64 turns (and freq * 2^-107): the error is position times that, at most about 2^-33
+// turns for freq below 2^42, and 2^-26 turns of rounding the angle to fp32. fp32 tensors take sincospif
+// of it, 16-bit ones the hardware's sine and cosine (absolute error at most 2^-21.1 on [-pi, pi],
+// beside the half step of 2^-9 or 2^-12 of the output). Everything else is fp32, rounded once.
 //
-// Bound: HBM (every element read once and written once) until the instructions count: a lane's head
-// costs about 280 of them per warp (16 elements: unpacking, norm, gains, rotation, packing, and its
-// share of addresses and cosines), which fill 58 % of the issue slots. Measured: 128 x 128 maps of 40
-// heads of 128, batch 4: 291 us, 4.6 TB/s, 71 % of the copy rate; keys of 5456 tokens, 8 heads of 32,
-// batch 32: 45 us, 4.0 TB/s; heads of 80 leave 3 of 8 lanes idle: 46 us, 3.2 TB/s. One to four heads
-// per lane and 8 to 32 warps per SM were measured; two and 16 are fastest.
+// Bound: latency, at 16 warps per SM with one step of loads in registers; neither HBM nor a pipe is
+// full. Four heads of 128 cost a warp 293 instructions (unpacking, norm, gains, rotation, packing,
+// and their share of addresses and cosines), which fill 58 % of the issue slots. Measured: 128 x
+// 128 maps of 40 heads of 128, batch 4: 293 us, 4.6 TB/s, 71 % of the copy rate; keys of 5456
+// tokens, 8 heads of 32, batch 32: 45 us, 4.0 TB/s; heads of 80 leave 3 of 8 lanes idle: 46 us, 3.2
+// TB/s. One to four heads per lane and 8 to 32 warps per SM were measured; two and 16 are fastest.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -28,8 +28,8 @@ DevInfo* current_device(int* dev) {
 
 cudaLaunchConfig_t launch_config(unsigned grid, unsigned threads, size_t smem, cudaStream_t st,
                                  cudaLaunchAttribute (&attr)[2], unsigned cluster) {
-  // may start while the kernel ahead of it finishes; all three kernels call griddep_wait before they
-  // touch memory
+  // may start while the kernel ahead of it finishes; all three kernels call griddep_wait before
+  // they touch memory
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -190,15 +190,16 @@ struct AttnPlan {
 // Limit of each wait of the tiled kernel; shorter ones are for tests of what happens behind it.
 std::atomic<unsigned long long> g_attn_wait_ns{kDefaultTimeoutNs};
 
-// States under a key mask, tiled kernel: the search of a longer row without a kept state would hold an
-// SM for more than 0.46 s per item.
+// States under a key mask, tiled kernel: the search of a longer row without a kept state would hold
+// an SM for more than 0.46 s per item.
 constexpr int kMaskTokens = 1 << 28;
 constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
 
-// CTAs of a cluster that split the states of one item, from the time of the whole in units of a state
-// tile (about 2 us: its MMAs and exponentials for both warpgroups): waves of clusters * (tiles of a
-// CTA + start + join). An item that is not split costs no join, and one start for all items of its
-// CTA. (18 items of 8 tiles, split 8: 15 of the clusters run at once, 26 us; split 4: 15 us.)
+// CTAs of a cluster that split the states of one item, from the time of the whole in units of a
+// state tile (about 2 us: its MMAs and exponentials for both warpgroups): waves of clusters *
+// (tiles of a CTA + start + join). An item that is not split costs no join, and one start for all
+// items of its CTA. (18 items of 8 tiles, split 8: 15 of the clusters run at once, 26 us; split 4:
+// 15 us.)
 int attn_split(int64_t items, int64_t tiles) {
   // clusters of 1, 2, ... CTAs that run at once with one CTA per SM, as the GPCs of 148 SMs allow
   static constexpr int kResident[kAttnMaxSplit + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
@@ -241,6 +242,10 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   const int group = d->q_heads / d->kv_heads;
   const int64_t rows = int64_t(d->q_tokens) * group;
   if (rows > INT_MAX - 2 * kAttnTile) return DCNV2_ERR_INVALID_ARG;
+  // The step kernel holds 16 rows. Where it can run it is the faster one (us, step / tiled): 8 x
+  // 60001 states, 8 kv heads of 128, 16 rows: 288 / 309; 32 x 5456, 8 heads of 32, 1 to 16 rows: 32
+  // / 88; 5456 states, 8 kv heads of 128, 4 and 16 rows: 11.2 / 15.2, 13.8 / 17.3. With one row
+  // more the tiled kernel takes those times: 310 (24 rows), 85 (17), 16.5 (20).
   p->step = rows <= kStepRows;
   if (p->step) {
     if (int64_t(d->batch) * d->kv_heads * kStepMaxSplit > INT_MAX) return DCNV2_ERR_INVALID_ARG;
@@ -250,6 +255,11 @@ dcnv2_status make_attn_plan(const dcnv2_attention_desc* d, AttnPlan* p) {
   for (p->heads = group < kAttnTile ? group : kAttnTile; group % p->heads;) --p->heads;
   p->kv_parts = group / p->heads;
   p->tile_tokens = kAttnTile / p->heads;
+  // One tile of rows: both warpgroups take its states in turn, or they would do nothing (us, paired
+  // / not): 8 x 60001 states, 8 kv heads of 128, 24 to 128 rows: 310-338 / 424-441; 32 x 5456, 8
+  // heads of 32, 17 to 128 rows: 85-90 / 189-191; 8 x 4001, 8 heads of 64: 22-26 / 43-45. Many
+  // items of few states are the exception (64 x 300, 8 heads of 128: 49-70 / 43-46): a paired CTA
+  // starts and joins anew for each.
   p->paired = d->q_tokens <= p->tile_tokens;
   p->wgs = !p->paired && !p->wide ? AttnLayout<64, false>::kWGs : AttnLayout<128, false>::kWGs;
   p->row_tiles =
@@ -287,7 +297,8 @@ bool encode_map(CUtensorMap* m, const void* p, int rank, const cuuint64_t* dims,
 
 // Tensor map of k or v: (element, token, head, batch), boxes of 64 elements x the 256 / wgs tokens
 // of a tile in the 128-byte swizzle. Axes that no step is taken along, or that share their states,
-// have extent 1. What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as zeros.
+// have extent 1. What lies outside (elements from head_dim on, tokens from kv_tokens on) reads as
+// zeros.
 bool states_map(CUtensorMap* m, const void* p, const int64_t (&stride)[3],
                 const dcnv2_attention_desc& d, int wgs, int* batch_step, int* head_step) {
   const bool heads = d.kv_heads > 1 && stride[2] > 0, batch = d.batch > 1 && stride[0] > 0;
@@ -361,12 +372,13 @@ dcnv2_status launch_attention(const AttnArgs& a, const AttnMaps& m, const AttnPl
                   : launch_attention<64, false, BF16>(a, m, p, dev, st);
 }
 
-// CTAs of a cluster that split the states of one (sequence, kv head): as few as give every SM a CTA,
-// with a chunk for each of their warps. One CTA draws at most about 50 GB/s, so that fewer CTAs than
-// SMs leave bandwidth unused, while more cost their start and end again (32 x 8 heads of 32, 5456
-// states: 256 CTAs 32 us, 512 36 us, 1024 44 us; 8 kv heads of 128, 5456 states: 64 CTAs 12.9 us, 128
-// 10.9 us). Lengths of their own leave SMs idle behind the short sequences; four times the CTAs even
-// that out (8 x 8 heads of 128, up to 60001 states: 128 CTAs 240 us, 512 208 us, 1024 200 us).
+// CTAs of a cluster that split the states of one (sequence, kv head): as few as give every SM a
+// CTA, with a chunk for each of their warps. One CTA draws at most about 50 GB/s, so that fewer
+// CTAs than SMs leave bandwidth unused, while more cost their start and end again (32 x 8 heads of
+// 32, 5456 states: 256 CTAs 32 us, 512 36 us, 1024 44 us; 8 kv heads of 128, 5456 states: 64 CTAs
+// 12.9 us, 128 10.9 us). Lengths of their own leave SMs idle behind the short sequences; four times
+// the CTAs even that out (8 x 8 heads of 128, up to 60001 states: 128 CTAs 240 us, 512 208 us, 1024
+// 200 us).
 int step_split(int64_t units, const AttnStepArgs& a, int sm_count) {
   const int keys = a.D > 64 ? 16 : a.D > 32 ? 32 : 64;
   const int64_t want = int64_t(sm_count) * (a.kv_lens ? 4 : 1);

@@ -16,9 +16,9 @@ namespace dcnv2 {
 // the thread until the phase completes; 0 spins (the MMA issuer, whose wake-up latency is on the
 // critical path). Waiting warps that do not spin leave the issue slots to the working ones.
 // CL selects a cluster-scope acquire (barriers that the peer CTA of a pair arrives on).
-// Where the wait is for a role whose own work may take long, `moved` is a count that this role steps
-// as it gets on: the time limit starts again, once, and then whenever the count has changed (it is
-// read only when the limit is over, so that a wait that ends in time costs nothing more).
+// Where the wait is for a role whose own work may take long, `moved` is a count that this role
+// steps as it gets on: the time limit starts again, once, and then whenever the count has changed
+// (it is read only when the limit is over, so that a wait that ends in time costs nothing more).
 constexpr int kSuspend = -1;
 struct WaitCtx {
   unsigned long long timeout_ns;
@@ -61,8 +61,8 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Wa
 }
 
 // The same wait for what a kernel itself still has in flight (copies, MMAs) before it ends or frees
-// tensor memory: neither an abort nor a shorter limit of the other waits cuts it short, only its own
-// limit, which no copy or MMA that still runs comes near.
+// tensor memory: neither an abort nor a shorter limit of the other waits cuts it short, only its
+// own limit, which no copy or MMA that still runs comes near.
 constexpr unsigned long long kDrainNs = 2000000000ull;
 __device__ __forceinline__ bool drain_bar(uint32_t bar, uint32_t parity, const WaitCtx& w) {
   const uint64_t t0 = ptx::global_timer_ns();
