@@ -193,7 +193,9 @@ std::atomic<unsigned long long> g_attn_wait_ns{kDefaultTimeoutNs};
 // States under a key mask, tiled kernel: the search of a longer row without a kept state would hold
 // an SM for more than 0.46 s per item.
 constexpr int kMaskTokens = 1 << 28;
-constexpr int kPlanSms = 148;     // SMs of the device the launch shapes are made for
+// SMs of the device that the launch shapes are made for. It is not asked: the workspace size, and the
+// words that an error is read from, follow from the desc alone, whatever device is current.
+constexpr int kPlanSms = 148;
 
 // CTAs of a cluster that split the states of one item, from the time of the whole in units of a
 // state tile (about 2 us: its MMAs and exponentials for both warpgroups): waves of clusters *
