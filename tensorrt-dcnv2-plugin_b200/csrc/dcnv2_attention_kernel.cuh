@@ -693,8 +693,10 @@ __global__ void __launch_bounds__((AttnLayout<DP, PAIRED>::kThreads), 1)
         for (int x = 2 * NW - 1; x > 1; x -= 2) top[0] = ptx::max3(top[0], top[x], top[x - 1]);
         top[0] = fmaxf(top[0], top[1]);
         const float m = fmaxf(m_ref, top[0]);
-        // (-inf) - (-inf) is NaN, which is not greater
-        if (__any_sync(0xffffffffu, (m - m_ref) * c > kAttnLazy)) {
+        // (-inf) - (-inf) is NaN, which is not greater. Rows behind the tile's last, whose Q is what
+        // shared memory held before (boxes of whole tokens may leave some of the 128), have no say:
+        // when the others are rescaled would depend on it, and with that their last bits.
+        if (__any_sync(0xffffffffu, live && (m - m_ref) * c > kAttnLazy)) {
           const float fac = m == m_ref ? 1.f : ptx::ex2((m_ref - m) * c);
           l *= fac;
           m_ref = m;

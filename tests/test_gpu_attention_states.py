@@ -107,3 +107,22 @@ def test_unkept_states_reach_nothing_in_any_form(b, L, h, g, d, bad):
     want, got = run(0.0), run(bad)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert bool(torch.isfinite(got[0]).all())
+
+
+@pytest.mark.parametrize("b,L,s,group,g,d", [
+    (5, 200, 191, 3, 1, 104), (3, 129, 3000, 33, 1, 96), (9, 300, 700, 7, 2, 64),
+    (2, 20, 3000, 5, 2, 128), (2, 20, 3000, 5, 2, 64), (90, 129, 256, 33, 1, 48),
+    (60, 290, 700, 3, 2, 128),
+])
+def test_bits_do_not_depend_on_what_ran_before(b, L, s, group, g, d):
+    """Groups of heads that leave rows of a tile unused, between calls that leave other values in an
+    SM's shared memory: the same bits every time."""
+    h = group * g
+    q = torch.randn(b, L, h, d, generator=gen(7), device=DEV).half()
+    k, v = (torch.randn(b, s, g, d, generator=gen(i), device=DEV).half() for i in (8, 9))
+    full = torch.randn(40, 1024, 8, d, generator=gen(10), device=DEV).half()
+    want = dcnv2_cross_attention(q, k, v, return_lse=True)
+    for scale in (100.0, -1000.0, 0.0, 30.0, math.nan, math.inf):
+        dcnv2_cross_attention(full * scale, full, full)
+        got = dcnv2_cross_attention(q, k, v, return_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
