@@ -287,9 +287,9 @@ DCNV2_API size_t dcnv2_cross_attention_workspace_size(const dcnv2_attention_desc
  *   lse       fp32 [batch][q_heads][q_tokens] or NULL: natural logarithm of the sum of the
  *   exponentials.
  * What states that are not kept hold (infinities, NaN) reaches no result. A sequence without any
- * kept state gives zeros and lse = -inf. Deterministic: the same call gives the same bits. Pointers
- * of q, k, v and out are 16-byte aligned device pointers of the current device; out overlaps no
- * input. Asynchronous on `stream`; never allocates or synchronises. The workspace needs no setting
+ * kept state, or a row whose kept scores are all -inf, gives zeros and lse = -inf. Deterministic:
+ * the same call gives the same bits. Pointers of q, k, v and out are 16-byte aligned device pointers
+ * of the current device; out overlaps no input. Asynchronous on `stream`; never allocates or synchronises. The workspace needs no setting
  * up, and calls that may overlap on the GPU need one each. Single tokens and few rows split the
  * states over a thread-block cluster. No counterpart in the reference plugin. */
 DCNV2_API dcnv2_status dcnv2_cross_attention(const dcnv2_attention_desc* desc, const void* q,

@@ -126,3 +126,30 @@ def test_bits_do_not_depend_on_what_ran_before(b, L, s, group, g, d):
         dcnv2_cross_attention(full * scale, full, full)
         got = dcnv2_cross_attention(q, k, v, return_lse=True)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("b,L,h,g,d", [(2, 1, 4, 2, 32), (2, 20, 4, 2, 64), (2, 300, 2, 2, 128),
+                                       (80, 130, 2, 2, 64)])
+def test_infinities_among_kept_states(b, L, h, g, d):
+    """Kept scores of -inf count as nothing: a row that has only those gives zeros and lse = -inf, one
+    that has others the result without them. NaN among the kept states shows in the rows that read it
+    and in no others."""
+    s = 300
+    q = torch.rand(b, L, h, d, generator=gen(11), device=DEV).half() + 0.5
+    k, v = (torch.randn(b, s, g, d, generator=gen(i), device=DEV).half() for i in (12, 13))
+    gone = torch.rand(b, s, generator=gen(14), device=DEV) < 0.3
+    gone[0] = True
+    low = torch.where(gone[:, :, None, None], torch.full((), -math.inf, dtype=FP16, device=DEV), k)
+    out, lse = dcnv2_cross_attention(q, low, v, return_lse=True)
+    want, want_lse = dcnv2_cross_attention(q, k, v, key_mask=~gone, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    assert not bool(out[0].any()) and bool((lse[0] == -math.inf).all())
+    v = v.clone()
+    v[-1, 5, 0, 3] = math.nan
+    k = k.clone()
+    k[1, 299, g - 1, 7] = math.nan
+    out = torch.isnan(dcnv2_cross_attention(q, k, v))
+    want = torch.zeros_like(out)
+    want[-1, :, :h // g, 3] = True
+    want[1, :, h - h // g:] = True
+    assert torch.equal(out, want)
