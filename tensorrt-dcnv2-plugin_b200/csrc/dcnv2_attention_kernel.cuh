@@ -41,7 +41,7 @@
 // Bound: at heads of 128, two row tiles times 128 states take 2756 cycles of MMAs (S, both
 // operands from shared memory: 102 cycles per 128 x 128 x 16; P V: 70) and 2048 of exponentials
 // (16 per clock and SM), and the chain of one row tile S -> P -> O -> next S takes 3250;
-// measured about 3680: 16 heads, 4096 x 16384: 541 us, 1.02 PFLOP/s (503 at best, 555-562 with
+// measured about 3680: 16 heads, 4096 x 16384: 541 us, 1.02 PFLOP/s (503 at best, 554-565 with
 // inputs that change from call to call), tensor pipe and exponentials 56 % busy each; 256 items on
 // 148 SMs are two rounds for 1.73 of work. At heads of 32 the MMAs are a quarter of that, and the
 // issuing warps' instructions (about 1150 cycles per row tile and 64 states: waits, six MMAs,
